@@ -713,3 +713,8 @@ def global_norm_squared(out, x, accumulate: bool = False) -> None:
             out[0] += val
         else:
             out[0] = val
+
+
+# ----------------------------------------------------------------------------- generation: 4-bit key/value cache, beam search
+from .beam import beam_select                                                                            # noqa: E402
+from .kv4 import KV4_PAGE, KV4Cache, attention_kv4, kv4_append, kv4_reorder, kv4_values                  # noqa: E402

@@ -1,0 +1,363 @@
+"""Key/value cache in 4 bits: write, read back, attention of new tokens over it, and its reordering by a beam search.
+
+The cache keeps keys and values in the form of the NVFP4 operands (``csrc/quant.cu``): e2m1 values, two to a byte with the first in the low
+nibble, and an e4m3 scale for every 16 values along the head; instead of a tensor scale, which would have to be known before the text is,
+there is one power of two for all keys and one for all values.  Every value that the cache can hold is then a bf16 number.
+
+    k_codes, v_codes    uint8 [layers, slots, kv_heads, capacity, head_size / 2]
+    k_scales, v_scales  uint8 [layers, slots, kv_heads, capacity, head_size / 16]
+
+A slot is one sequence.  ``capacity`` is a multiple of the ``KV4_PAGE`` = 64 tokens of a page; ``pages`` (int32 [slots, capacity / 64], optional)
+names for each slot and page the slot in whose place that page is kept, so that beams share the pages they have in common.  The page that a
+slot is filling, and those behind it, are always its own.
+
+CUDA tensors run ``csrc/kv4.cu`` and ``csrc/attention_kv4.cu``; CPU tensors run the fp32 PyTorch statement of the same definitions.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional
+
+import torch
+
+from . import _lib
+from ._lib import check, dtype_code, lib, ptr, status_word
+
+KV4_PAGE = 64
+KV4_UNIT = 2.0 ** -4          # largest value 2688 / 16 = 168; scales of 2^-6 and more (values of 0.006 and more) have all their bits
+KV4_HEAD_SIZES = (32, 64, 80, 96, 128)
+_LEVELS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+class _Kv4Desc(ctypes.Structure):
+    """``Kv4Desc`` of ``csrc/kv4.cuh``."""
+    _fields_ = [("kc", ctypes.c_void_p), ("ks", ctypes.c_void_p), ("vc", ctypes.c_void_p), ("vs", ctypes.c_void_p),
+                ("code_layer", ctypes.c_longlong), ("code_slot", ctypes.c_longlong),
+                ("scale_layer", ctypes.c_longlong), ("scale_slot", ctypes.c_longlong),
+                ("layers", ctypes.c_int), ("slots", ctypes.c_int), ("heads", ctypes.c_int), ("capacity", ctypes.c_int),
+                ("head_size", ctypes.c_int), ("k_exp", ctypes.c_int), ("v_exp", ctypes.c_int), ("pad", ctypes.c_int)]
+
+
+def _exponent(unit: float, name: str) -> int:
+    m, e = math.frexp(unit) if isinstance(unit, (int, float)) and math.isfinite(unit) else (0.0, 0)
+    if m != 0.5 or not -32 <= e - 1 <= 32:
+        raise ValueError(f"{name} must be a power of two between 2^-32 and 2^32, not {unit!r}")
+    return e - 1
+
+
+class KV4Cache:
+    """The four tensors of a cache (see the module), checked once.  Layers and slots may be strided views of larger caches (every third
+    slot, some of the layers); heads, tokens and values lie densely, every row 16-byte aligned."""
+
+    __slots__ = ("k_codes", "k_scales", "v_codes", "v_scales", "k_unit", "v_unit", "layers", "slots", "kv_heads", "capacity", "head_size",
+                 "device", "_desc", "_ref")
+
+    def __init__(self, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor,
+                 k_unit: float = KV4_UNIT, v_unit: float = KV4_UNIT):
+        if k_codes.dim() != 5:
+            raise ValueError(f"codes are [layers, slots, kv_heads, capacity, head_size / 2], not {tuple(k_codes.shape)}")
+        L, S, H, T, half = k_codes.shape
+        if 2 * half not in KV4_HEAD_SIZES:
+            raise ValueError(f"head size {2 * half}: the cache takes {KV4_HEAD_SIZES}")
+        if T % KV4_PAGE or T == 0 or min(L, S, H) == 0:
+            raise ValueError(f"capacity {T} must be a multiple of {KV4_PAGE}, and no dimension of {tuple(k_codes.shape)} empty")
+        if H > 65535 or S > 65535:
+            raise ValueError(f"at most 65535 slots and heads, not {S} and {H}")
+        codes, scales = (L, S, H, T, half), (L, S, H, T, half // 8)
+        dev = k_codes.device
+        cs, ss = k_codes.stride(), k_scales.stride()
+        for name, t, shape, strides in (("k_codes", k_codes, codes, cs), ("k_scales", k_scales, scales, ss),
+                                        ("v_codes", v_codes, codes, cs), ("v_scales", v_scales, scales, ss)):
+            if t.dtype != torch.uint8 or tuple(t.shape) != shape or t.device != dev:
+                raise ValueError(f"{name} must be uint8 {shape} on {dev}, not {t.dtype} {tuple(t.shape)} on {t.device}")
+            c = shape[4]
+            st = t.stride()
+            if st != strides:
+                raise ValueError(f"{name}: keys and values must have the same strides, not {st} and {strides}")
+            if st[4] != 1 or st[3] != c or (H > 1 and st[2] != T * c) or (t.data_ptr() | (st[1] if S > 1 else 0) | (st[0] if L > 1 else 0)) % 16:
+                raise ValueError(f"{name}: heads, tokens and values must lie densely, slots and layers 16-byte aligned (strides {st})")
+            if (S > 1 and st[1] < H * T * c) or (L > 1 and st[0] < H * T * c):
+                raise ValueError(f"{name}: slots and layers must not overlap (strides {st})")
+        self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
+        self.k_unit, self.v_unit = k_unit, v_unit
+        self.layers, self.slots, self.kv_heads, self.capacity, self.head_size, self.device = L, S, H, T, 2 * half, dev
+        self._desc = _Kv4Desc(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), cs[0], cs[1], ss[0], ss[1],
+                              L, S, H, T, 2 * half, _exponent(k_unit, "k_unit"), _exponent(v_unit, "v_unit"), 0)
+        self._ref = ctypes.addressof(self._desc)
+
+    @classmethod
+    def empty(cls, layers: int, slots: int, kv_heads: int, max_len: int, head_size: int, device="cuda", k_unit: float = KV4_UNIT,
+              v_unit: float = KV4_UNIT) -> "KV4Cache":
+        """A cache for ``slots`` sequences of up to ``max_len`` tokens, all zeros."""
+        if head_size not in KV4_HEAD_SIZES:
+            raise ValueError(f"head size {head_size}: the cache takes {KV4_HEAD_SIZES}")
+        T = max(1, -(-max_len // KV4_PAGE)) * KV4_PAGE
+        z = lambda c: torch.zeros(layers, slots, kv_heads, T, c, dtype=torch.uint8, device=device)  # noqa: E731
+        return cls(z(head_size // 2), z(head_size // 16), z(head_size // 2), z(head_size // 16), k_unit, v_unit)
+
+    def own_pages(self) -> torch.Tensor:
+        """The page table in which every page lies in its own slot."""
+        return torch.arange(self.slots, dtype=torch.int32, device=self.device).view(-1, 1).repeat(1, self.capacity // KV4_PAGE)
+
+    def select(self, slots: slice) -> "KV4Cache":
+        """The same cache restricted to some of its slots (a slice): a view."""
+        return KV4Cache(self.k_codes[:, slots], self.k_scales[:, slots], self.v_codes[:, slots], self.v_scales[:, slots], self.k_unit, self.v_unit)
+
+    def nbytes(self) -> int:
+        return self.layers * self.slots * self.kv_heads * self.capacity * (self.head_size // 2 + self.head_size // 16) * 2
+
+
+# ------------------------------------------------------------------ arguments
+class _on:
+    """Launches go to the current stream of the tensors' device, whichever device is current."""
+    __slots__ = ("guard", "stream")
+
+    def __init__(self, device: torch.device):
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self) -> int:
+        if self.guard is not None:
+            self.guard.__enter__()
+        return _lib.stream()
+
+    def __exit__(self, *e):
+        if self.guard is not None:
+            self.guard.__exit__(*e)
+
+
+def _ints(t: Optional[torch.Tensor], name: str, shape: tuple, device) -> None:
+    if t is None:
+        return
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 {shape} on {device}, not {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _layer(cache: KV4Cache, layer: int) -> int:
+    if not isinstance(layer, int) or not 0 <= layer < cache.layers:
+        raise ValueError(f"layer {layer!r} of a cache of {cache.layers} layers")
+    return layer
+
+
+def _rows(t: torch.Tensor, name: str, shape: tuple, dtype, device) -> None:
+    if t.dtype != dtype or tuple(t.shape) != shape or t.device != device:
+        raise ValueError(f"{name} must be {dtype} {shape} on {device}, not {t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.numel() and t.stride(-1) != 1:
+        raise ValueError(f"{name}: the values of a head must lie densely (strides {t.stride()})")
+
+
+def _spread(t: torch.Tensor, name: str) -> None:
+    """An output whose elements share memory would be written by several threads."""
+    span = 1
+    for n, s in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n > 1), key=lambda p: p[1]):
+        if s < span:
+            raise ValueError(f"{name}: elements of an output must not overlap (shape {tuple(t.shape)}, strides {t.stride()})")
+        span = s * n
+
+
+def _count(n: int = 1) -> None:
+    from .. import ops
+    ops._count(n)
+
+
+# ------------------------------------------------------------------ the definitions, on any device, in fp32
+def _encode(x: torch.Tensor, unit: float):
+    """(codes, scales) of x [..., head_size]: a block's scale is e4m3(amax / 6 / unit), its values e2m1(x / (scale unit)), ties to even."""
+    b = x.float().unflatten(-1, (-1, 16))
+    scale = (b.abs().amax(-1, keepdim=True) / unit / 6.0).nan_to_num(0.0, 448.0, 448.0).clamp(max=448.0).to(torch.float8_e4m3fn)
+    s = scale.float() * unit
+    t = torch.where(s > 0, b.abs() / s, torch.zeros_like(b))
+    code = sum(((t > e) if i % 2 == 0 else (t >= e)).to(torch.uint8) for i, e in enumerate((0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0)))
+    code = (code | torch.signbit(b).to(torch.uint8) << 3).flatten(-2)
+    return code[..., 0::2] | code[..., 1::2] << 4, scale.view(torch.uint8).squeeze(-1)
+
+
+def _decode(codes: torch.Tensor, scales: torch.Tensor, unit: float) -> torch.Tensor:
+    code = torch.stack([codes & 15, codes >> 4], -1).flatten(-2).long()
+    level = torch.tensor(_LEVELS + tuple(-v for v in _LEVELS), device=codes.device)[code]
+    return (level.unflatten(-1, (-1, 16)) * (scales.view(torch.float8_e4m3fn).float() * unit).unsqueeze(-1)).flatten(-2)
+
+
+# ------------------------------------------------------------------ operators
+def kv4_append(cache: KV4Cache, layer: int, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor,
+               counts: Optional[torch.Tensor] = None) -> None:
+    """Writes keys and values ``k``, ``v`` [slots, n, kv_heads, head_size] (bf16 or fp32; strided views of a packed qkv, for instance) of
+    ``n`` new tokens to the positions ``start[s] + i`` of one layer.  ``counts`` [slots]: the first ``counts[s]`` of them only (prompts padded
+    to one shape).  Positions outside the cache are not written.  ``start`` and ``counts`` are int32 on the device.
+
+    A value beyond the largest one (2688 units) becomes that one.  A token and head with a non-finite key or value has no 4-bit form: its
+    key and its value are kept as NaN, and every query that sees it answers NaN."""
+    S, n, H, hd = k.shape if k.dim() == 4 else (None,) * 4
+    if (S, H, hd) != (cache.slots, cache.kv_heads, cache.head_size):
+        raise ValueError(f"k must be [{cache.slots}, n, {cache.kv_heads}, {cache.head_size}], not {tuple(k.shape)}")
+    if k.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"k and v must be bf16 or fp32, not {k.dtype}")
+    _layer(cache, layer)
+    _rows(k, "k", (S, n, H, hd), k.dtype, cache.device)
+    _rows(v, "v", (S, n, H, hd), k.dtype, cache.device)
+    _ints(start, "start", (S,), cache.device)
+    _ints(counts, "counts", (S,), cache.device)
+    if n == 0:
+        return
+    if k.is_cuda:
+        ks, vs = k.stride(), v.stride()
+        with _on(cache.device) as stream:
+            check(lib().llmb_kv4_append(cache._ref, layer, ptr(k), ptr(v), ptr(start), ptr(counts), n, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+                                        dtype_code(k), stream), "kv4_append")
+        _count()
+        return
+    kf, vf = k.float(), v.float()
+    bad = ~(torch.isfinite(kf).all(-1, keepdim=True) & torch.isfinite(vf).all(-1, keepdim=True))
+    for s in range(S):
+        p0 = int(start[s])
+        lo, hi = max(0, -p0), min(n if counts is None else min(n, int(counts[s])), cache.capacity - p0)
+        if lo >= hi:
+            continue
+        for x, codes, scales, unit in ((kf, cache.k_codes, cache.k_scales, cache.k_unit), (vf, cache.v_codes, cache.v_scales, cache.v_unit)):
+            c, f = _encode(x[s, lo:hi].nan_to_num(0.0, 0.0, 0.0), unit)
+            f = torch.where(bad[s, lo:hi], torch.full_like(f, 0x7f), f)
+            codes[layer, s, :, p0 + lo:p0 + hi] = c.transpose(0, 1)
+            scales[layer, s, :, p0 + lo:p0 + hi] = f.transpose(0, 1)
+
+
+def kv4_values(k_out: torch.Tensor, v_out: torch.Tensor, cache: KV4Cache, layer: Optional[int], start: torch.Tensor,
+               pages: Optional[torch.Tensor] = None) -> None:
+    """Reads back what the cache holds: ``k_out``, ``v_out`` [slots, n, kv_heads, head_size] (bf16, in which every value is exact, or fp32) of
+    the positions ``start[s] + i`` of one layer, or [layers, slots, ...] of all layers (``layer`` None).  Positions outside the cache read as
+    zeros, pages whose entry in ``pages`` names no slot as NaN."""
+    lead = (cache.layers, cache.slots) if layer is None else (cache.slots,)
+    n = k_out.shape[-3] if k_out.dim() == len(lead) + 3 else -1
+    shape = (*lead, n, cache.kv_heads, cache.head_size)
+    if k_out.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"k_out and v_out must be bf16 or fp32, not {k_out.dtype}")
+    if layer is not None:
+        _layer(cache, layer)
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        _rows(t, name, shape, k_out.dtype, cache.device)
+        _spread(t, name)
+        if layer is None and t.numel() and t.stride() != k_out.stride():
+            raise ValueError(f"k_out and v_out must have the same strides, not {k_out.stride()} and {t.stride()}")
+    _ints(start, "start", (cache.slots,), cache.device)
+    _ints(pages, "pages", (cache.slots, cache.capacity // KV4_PAGE), cache.device)
+    if n == 0:
+        return
+    if k_out.is_cuda:
+        ks, vs = k_out.stride(), v_out.stride()
+        with _on(cache.device) as stream:
+            check(lib().llmb_kv4_values(cache._ref, -1 if layer is None else layer, ptr(k_out), ptr(v_out), ptr(start), ptr(pages), n,
+                                        ks[0] if layer is None else 0, *ks[-4:-1], *vs[-4:-1], dtype_code(k_out), stream), "kv4_values")
+        _count()
+        return
+    T, i = cache.capacity, torch.arange(n)
+    for s in range(cache.slots):
+        pos = int(start[s]) + i
+        inside = (pos >= 0) & (pos < T)
+        pos = pos.clamp(0, T - 1)
+        slot = torch.full_like(pos, s) if pages is None else pages[s].long()[pos // KV4_PAGE]
+        wrong = (slot < 0) | (slot >= cache.slots)
+        slot = slot.clamp(0, cache.slots - 1)
+        for l in range(cache.layers) if layer is None else (layer,):
+            for out, codes, scales, unit in ((k_out, cache.k_codes, cache.k_scales, cache.k_unit), (v_out, cache.v_codes, cache.v_scales, cache.v_unit)):
+                x = _decode(codes[l, slot, :, pos], scales[l, slot, :, pos], unit)
+                x[wrong] = float("nan")
+                x[~inside] = 0.0
+                (out[l] if layer is None else out)[s] = x.to(out.dtype)
+
+
+def attention_kv4(out: torch.Tensor, q: torch.Tensor, cache: KV4Cache, layer: int, lens: torch.Tensor, counts: Optional[torch.Tensor] = None,
+                  pages: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> None:
+    """Attention of the newest tokens of each slot over one layer of the cache (their own keys and values are in it already).
+
+    ``q``, ``out`` [slots, n, heads, head_size], bf16 or fp32, strided views allowed, ``heads`` a multiple of the cache's; head h reads key head
+    h // (heads / kv_heads).  ``lens`` [slots]: tokens in the cache; ``counts`` [slots]: how many of the n rows of a slot are queries (n without
+    it).  Row i < counts[s] is the token at position lens[s] - counts[s] + i and sees the positions up to its own; a row that sees none (an
+    empty slot) gives zeros; rows behind counts[s] are left as they are.  ``scale``: of the scores, 1 / sqrt(head_size) by default.
+    ``out`` may be ``q`` itself.  A page whose entry in ``pages`` names no slot gives NaN to every row that sees it.
+
+    Scores, statistics and sums are in fp32.  lens above the capacity count as the capacity."""
+    if q.dim() != 4 or (q.shape[0], q.shape[3]) != (cache.slots, cache.head_size) or q.shape[2] % cache.kv_heads or q.shape[2] == 0:
+        raise ValueError(f"q must be [{cache.slots}, n, a multiple of {cache.kv_heads}, {cache.head_size}], not {tuple(q.shape)}")
+    if q.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"q must be bf16 or fp32, not {q.dtype}")
+    S, n, heads, hd = q.shape
+    _layer(cache, layer)
+    _rows(q, "q", (S, n, heads, hd), q.dtype, cache.device)
+    _rows(out, "out", (S, n, heads, hd), q.dtype, cache.device)
+    _spread(out, "out")
+    _ints(lens, "lens", (S,), cache.device)
+    _ints(counts, "counts", (S,), cache.device)
+    _ints(pages, "pages", (S, cache.capacity // KV4_PAGE), cache.device)
+    scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be finite, not {scale}")
+    if n * (heads // cache.kv_heads) > 2 ** 30:
+        raise ValueError(f"{n} rows of {heads} heads are too many")
+    if n == 0:
+        return
+    if q.is_cuda:
+        qs, os_ = q.stride(), out.stride()
+        with _on(cache.device) as stream:
+            check(lib().llmb_attention_kv4(cache._ref, layer, ptr(out), ptr(q), ptr(lens), ptr(counts), ptr(pages), n, heads, scale,
+                                           qs[0], qs[1], qs[2], os_[0], os_[1], os_[2], dtype_code(q), ptr(status_word(cache.device)), stream),
+                  "attention_kv4")
+        _count()
+        return
+    group, T = heads // cache.kv_heads, cache.capacity
+    for s in range(S):
+        L = min(max(int(lens[s]), 0), T)
+        c = n if counts is None else min(max(int(counts[s]), 0), n)
+        if c == 0:
+            continue
+        pos = torch.arange(L)
+        slot = torch.full_like(pos, s) if pages is None else pages[s].long()[pos // KV4_PAGE]
+        wrong = (slot < 0) | (slot >= cache.slots)
+        slot = slot.clamp(0, cache.slots - 1)
+        k = _decode(cache.k_codes[layer, slot, :, pos], cache.k_scales[layer, slot, :, pos], cache.k_unit)      # [L, H, hd]
+        v = _decode(cache.v_codes[layer, slot, :, pos], cache.v_scales[layer, slot, :, pos], cache.v_unit)
+        k[wrong] = float("nan")
+        v = v.nan_to_num(0.0)                    # such a token's key is NaN as well: its weight says so to the rows that see it
+        x = q[s, :c].float().view(c, cache.kv_heads, group, hd)
+        w = torch.einsum("chgd,lhd->hgcl", x, k) * scale
+        w = w.masked_fill(pos.view(1, -1) >= (L - c + 1 + torch.arange(c)).view(-1, 1), float("-inf"))
+        m = w.amax(-1, keepdim=True) if L else torch.zeros(*w.shape[:-1], 1)
+        p = torch.exp(w - torch.where(torch.isneginf(m), torch.zeros_like(m), m))
+        total = p.sum(-1, keepdim=True)
+        o = torch.einsum("hgcl,lhd->chgd", p / torch.where(total == 0, torch.ones_like(total), total), v)
+        out[s, :c] = o.reshape(c, heads, hd).to(out.dtype)
+
+
+def kv4_reorder(cache: KV4Cache, pages: torch.Tensor, lens: torch.Tensor, parents: torch.Tensor) -> None:
+    """The cache follows a beam search: slot b K + j of item b becomes what slot b K + ``parents[b, j]`` was (``parents`` int32 [items, K],
+    items x K = slots), in place and in every layer.  Entries of ``pages`` for whole pages and ``lens`` are permuted; of the keys and values
+    only the page that is being filled is copied, at most 63 tokens.  Entries for pages that are not full name the slot itself.  A parent
+    outside 0 .. K - 1 counts as j itself; lengths beyond the capacity count as the capacity.
+
+    A full page is never written again, so any number of slots may share it; the tokens appended next go to the slot's own place."""
+    if parents.dim() != 2 or parents.numel() != cache.slots or parents.shape[1] == 0:
+        raise ValueError(f"parents must be [items, K] with items x K = {cache.slots}, not {tuple(parents.shape)}")
+    B, K = parents.shape
+    if K > 64:
+        raise ValueError(f"at most 64 beams, not {K}")
+    _ints(parents, "parents", (B, K), cache.device)
+    _ints(lens, "lens", (cache.slots,), cache.device)
+    _ints(pages, "pages", (cache.slots, cache.capacity // KV4_PAGE), cache.device)
+    if pages is None or lens is None:
+        raise ValueError("kv4_reorder permutes pages and lens: both are needed")
+    if lens.is_cuda:
+        with _on(cache.device) as stream:
+            check(lib().llmb_kv4_reorder(cache._ref, ptr(pages), ptr(lens), ptr(parents), K, stream), "kv4_reorder")
+        _count(2)
+        return
+    slot = torch.arange(cache.slots)
+    j = parents.flatten().long()
+    src = torch.where((j < 0) | (j >= K), slot, slot // K * K + j)
+    new = lens[src].clamp(0, cache.capacity)
+    full = new // KV4_PAGE
+    old = [t.clone() for t in (cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales)]
+    for s in range(cache.slots):
+        a, z = int(full[s]) * KV4_PAGE, int(new[s])
+        for t, o in zip((cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales), old):
+            t[:, s, :, a:z] = o[:, src[s], :, a:z]
+    whole = torch.arange(pages.shape[1]) < full.view(-1, 1)
+    pages.copy_(torch.where(whole, pages[src], slot.view(-1, 1).int()))
+    lens.copy_(new)

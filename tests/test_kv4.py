@@ -1,0 +1,201 @@
+"""The 4-bit key/value cache and the beam selection on CPU tensors: definitions against 64-bit statements, and what is refused."""
+import math
+
+import pytest
+import torch
+
+from kv4_oracle import Dense, attention64, rounded64, select64
+from llm_mojo_b200 import ops
+
+
+def rnd(*shape, dtype=torch.float32, scale=1.0, seed=0):
+    g = torch.Generator().manual_seed(seed + 13 * sum(shape))
+    return (torch.randn(*shape, generator=g) * scale).to(dtype)
+
+
+def i32(*v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("hd", ops.kv4.KV4_HEAD_SIZES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_append_then_values_is_the_rounding(hd, dtype):
+    c = ops.KV4Cache.empty(2, 3, 2, 100, hd, "cpu")
+    k, v = rnd(3, 5, 2, hd, dtype=dtype, scale=3.0), rnd(3, 5, 2, hd, dtype=dtype, scale=0.01, seed=1)
+    ops.kv4_append(c, 1, k, v, i32(0, 60, 125), counts=i32(5, 5, 5))
+    ko, vo = torch.empty_like(k), torch.empty_like(v)
+    ops.kv4_values(ko, vo, c, 1, i32(0, 60, 125))
+    for got, x in ((ko, k), (vo, v)):
+        want = rounded64(x, ops.kv4.KV4_UNIT)
+        want[2, 3:] = 0.0                                    # positions 128, 129 of a capacity of 128
+        assert torch.equal(got.double(), want)
+    assert not c.k_codes[0].any() and not c.v_scales[0].any()
+
+
+def test_attention_is_causal_and_rows_behind_the_counts_stay():
+    c = ops.KV4Cache.empty(1, 2, 2, 64, 32, "cpu")
+    d = Dense(2, 2, 64, 32)
+    k, v = rnd(2, 9, 2, 32), rnd(2, 9, 2, 32, seed=1)
+    ops.kv4_append(c, 0, k, v, i32(0, 0), counts=i32(9, 4))
+    d.append(k, v, [0, 0], [9, 4])
+    q = rnd(2, 5, 6, 32, seed=2)
+    out = torch.full_like(q, 7.0)
+    ops.attention_kv4(out, q, c, 0, i32(9, 4), counts=i32(5, 3))
+    want, _ = attention64(q, d, [9, 4], [5, 3])
+    assert torch.allclose(out[0].double(), want[0], atol=1e-5) and torch.allclose(out[1, :3].double(), want[1, :3], atol=1e-5)
+    assert (out[1, 3:] == 7.0).all()
+
+
+def test_reorder_follows_dense_copies_of_the_beams():
+    items, K, H, hd, T = 2, 3, 2, 32, 192
+    S = items * K
+    c, d = ops.KV4Cache.empty(2, S, H, T, hd, "cpu"), Dense(S, H, T, hd)
+    pages, lens = c.own_pages(), torch.zeros(S, dtype=torch.int32)
+    g = torch.Generator().manual_seed(3)
+    for step, n in enumerate((50, 14, 1, 63, 2, 30)):
+        k, v = rnd(S, n, H, hd, seed=step), rnd(S, n, H, hd, seed=100 + step)
+        for l in range(2):
+            ops.kv4_append(c, l, k, v, lens)
+        d.append(k, v, lens.tolist(), [n] * S)
+        lens += n
+        parents = torch.randint(0, K, (items, K), generator=g, dtype=torch.int32)
+        ops.kv4_reorder(c, pages, lens, parents)
+        d.reorder([b * K + p for b, row in enumerate(parents.tolist()) for p in row])
+        L = int(lens[0])
+        ko, vo = torch.empty(2, S, L, H, hd), torch.empty(2, S, L, H, hd)
+        ops.kv4_values(ko, vo, c, None, torch.zeros(S, dtype=torch.int32), pages)
+        assert torch.equal(ko[1].double(), d.k[:, :L]) and torch.equal(vo[0].double(), d.v[:, :L])
+
+
+@pytest.mark.parametrize("K,V", [(1, 5), (4, 4), (3, 50), (8, 5000)])
+def test_beam_select_is_the_definition(K, V):
+    B = 3
+    logits = rnd(B * K, V + 3, dtype=torch.bfloat16, scale=2.0)
+    scores = -rnd(B, K).abs()
+    finished = torch.rand(B, K, generator=torch.Generator().manual_seed(1)) < 0.3
+    so, t, p, f = torch.empty(B, K), torch.empty(B, K, dtype=torch.int32), torch.empty(B, K, dtype=torch.int32), torch.empty(B, K, dtype=torch.bool)
+    ops.beam_select(so, t, p, logits, scores, V, finished_out=f, finished=finished, eos=2)
+    w = select64(logits, scores, V, finished, 2)
+    assert torch.equal(t.long(), w[1]) and torch.equal(p.long(), w[2]) and torch.equal(f, w[3])
+    assert torch.allclose(so.double(), w[0], rtol=1e-6)
+
+
+def _cache(**kw):
+    a = dict(layers=1, slots=2, kv_heads=2, max_len=64, head_size=64, device="cpu")
+    return ops.KV4Cache.empty(**{**a, **kw})
+
+
+def test_cache_refusals():
+    c = _cache()
+    t = (c.k_codes, c.k_scales, c.v_codes, c.v_scales)
+    with pytest.raises(ValueError, match="head size"):
+        _cache(head_size=72)
+    with pytest.raises(ValueError, match="power of two"):
+        ops.KV4Cache(*t, k_unit=0.1)
+    with pytest.raises(ValueError, match="power of two"):
+        ops.KV4Cache(*t, v_unit=float("nan"))
+    with pytest.raises(ValueError, match="k_scales"):
+        ops.KV4Cache(t[0], t[1][..., :2], t[2], t[3])
+    with pytest.raises(ValueError, match="v_codes"):
+        ops.KV4Cache(t[0], t[1], t[2].to(torch.int8), t[3])
+    with pytest.raises(ValueError, match="capacity"):
+        ops.KV4Cache(*(x[:, :, :, :32] for x in t))
+    with pytest.raises(ValueError, match="densely"):
+        ops.KV4Cache(*(x.transpose(1, 2).contiguous().transpose(1, 2) for x in t))
+    with pytest.raises(ValueError, match="overlap"):
+        ops.KV4Cache(*(x[:, :1].expand(1, 2, *x.shape[2:]) for x in t))
+    with pytest.raises(ValueError, match="layers"):
+        ops.KV4Cache(*(x[0] for x in t))
+    assert c.select(slice(0, None, 2)).slots == 1
+
+
+def test_append_and_values_refusals():
+    c, x, z = _cache(), torch.zeros(2, 3, 2, 64), i32(0, 0)
+    for bad in (torch.zeros(2, 3, 2, 32), torch.zeros(1, 3, 2, 64), torch.zeros(2, 3, 64)):
+        with pytest.raises(ValueError):
+            ops.kv4_append(c, 0, bad, bad, z)
+    with pytest.raises(TypeError):
+        ops.kv4_append(c, 0, x.half(), x.half(), z)
+    with pytest.raises(ValueError, match="v must be"):
+        ops.kv4_append(c, 0, x, x.bfloat16(), z)
+    with pytest.raises(ValueError, match="densely"):
+        ops.kv4_append(c, 0, torch.zeros(2, 3, 2, 128)[..., ::2], x, z)
+    with pytest.raises(ValueError, match="layer"):
+        ops.kv4_append(c, 1, x, x, z)
+    with pytest.raises(ValueError, match="start"):
+        ops.kv4_append(c, 0, x, x, z.long())
+    with pytest.raises(ValueError, match="counts"):
+        ops.kv4_append(c, 0, x, x, z, counts=i32(1))
+    with pytest.raises(ValueError, match="overlap"):
+        ops.kv4_values(torch.zeros(2, 1, 2, 64).expand(2, 3, 2, 64), x, c, 0, z)
+    with pytest.raises(ValueError, match="k_out"):
+        ops.kv4_values(x, x.clone(), c, None, z)
+    with pytest.raises(ValueError, match="pages"):
+        ops.kv4_values(x, x.clone(), c, 0, z, pages=torch.zeros(2, 2, dtype=torch.int32))
+    ops.kv4_append(c, 0, x[:, :0], x[:, :0], z)              # nothing to do is no error
+
+
+def test_attention_refusals():
+    c, q, n = _cache(), torch.zeros(2, 1, 4, 64), i32(1, 1)
+    for bad in (torch.zeros(2, 1, 3, 64), torch.zeros(2, 1, 4, 32), torch.zeros(3, 1, 4, 64), torch.zeros(2, 4, 64), torch.zeros(2, 1, 0, 64)):
+        with pytest.raises(ValueError, match="q must be"):
+            ops.attention_kv4(bad.clone(), bad, c, 0, n)
+    with pytest.raises(TypeError):
+        ops.attention_kv4(q.half(), q.half(), c, 0, n)
+    with pytest.raises(ValueError, match="out must be"):
+        ops.attention_kv4(q.bfloat16(), q, c, 0, n)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.attention_kv4(torch.zeros(1, 1, 4, 64).expand(2, 1, 4, 64), q, c, 0, n)
+    with pytest.raises(ValueError, match="lens"):
+        ops.attention_kv4(q.clone(), q, c, 0, torch.ones(2, 2, dtype=torch.int32)[:, 0])
+    with pytest.raises(ValueError, match="scale"):
+        ops.attention_kv4(q.clone(), q, c, 0, n, scale=float("inf"))
+    with pytest.raises(ValueError, match="layer"):
+        ops.attention_kv4(q.clone(), q, c, -1, n)
+
+
+def test_reorder_and_select_refusals():
+    c = _cache(slots=6)
+    pages, lens, par = c.own_pages(), torch.zeros(6, dtype=torch.int32), torch.zeros(2, 3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="parents"):
+        ops.kv4_reorder(c, pages, lens, par[:1])
+    with pytest.raises(ValueError, match="parents"):
+        ops.kv4_reorder(c, pages, lens, par.long())
+    with pytest.raises(ValueError, match="pages"):
+        ops.kv4_reorder(c, pages[:, :0], lens, par)
+    with pytest.raises(ValueError, match="needed"):
+        ops.kv4_reorder(c, None, lens, par)
+    so, t, p = torch.empty(2, 3), par.clone(), par.clone()
+    x, s = torch.zeros(6, 10), torch.zeros(2, 3)
+    with pytest.raises(ValueError, match="logits"):
+        ops.beam_select(so, t, p, x[:5], s, 10)
+    with pytest.raises(ValueError, match="vocabulary"):
+        ops.beam_select(so, t, p, x, s, 11)
+    with pytest.raises(ValueError, match="vocabulary"):
+        ops.beam_select(so, t, p, x, s, 2)                   # fewer tokens than beams
+    with pytest.raises(ValueError, match="eos"):
+        ops.beam_select(so, t, p, x, s, 10, eos=10)
+    with pytest.raises(ValueError, match="eos"):
+        ops.beam_select(so, t, p, x, s, 10, finished=torch.zeros(2, 3, dtype=torch.bool))
+    with pytest.raises(ValueError, match="share"):
+        ops.beam_select(s, t, p, x, s, 10)
+    with pytest.raises(ValueError, match="share"):
+        ops.beam_select(so, t, t, x, s, 10)
+    with pytest.raises(ValueError, match="tokens"):
+        ops.beam_select(so, t.long(), p, x, s, 10)
+    with pytest.raises(TypeError):
+        ops.beam_select(so, t, p, x.half(), s, 10)
+    with pytest.raises(ValueError, match="beams"):
+        ops.beam_select(torch.empty(1, 65), torch.empty(1, 65, dtype=torch.int32), torch.empty(1, 65, dtype=torch.int32), torch.zeros(65, 100),
+                        torch.zeros(1, 65), 100)
+
+
+def test_a_row_that_is_not_finite_is_kept_as_nan_and_seen_by_no_one_else():
+    c = ops.KV4Cache.empty(1, 1, 1, 64, 32, "cpu")
+    k, v = rnd(1, 6, 1, 32), rnd(1, 6, 1, 32, seed=1)
+    v[0, 4, 0, 20] = float("inf")
+    ops.kv4_append(c, 0, k, v, i32(0))
+    q = rnd(1, 6, 1, 32, seed=2)
+    out = torch.empty_like(q)
+    ops.attention_kv4(out, q, c, 0, i32(6))
+    assert torch.isfinite(out[0, :4]).all() and torch.isnan(out[0, 4:]).all()
