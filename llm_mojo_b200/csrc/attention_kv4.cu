@@ -447,10 +447,18 @@ int run_type(const Kv4Attn& p, cudaStream_t st) {
 }
 }  // namespace
 
-LLMB_API int llmb_attention_kv4(const Kv4Desc* d, int layer, void* out, const void* q, const int* lens, const int* counts, const int* pages, int n, int heads,
-                                float scale, long long qb, long long qt, long long qh, long long ob, long long ot, long long oh, int dtype, int* status,
-                                cudaStream_t st) {
-  if (heads % d->heads || d->heads > 65535 || d->slots > 65535) return LLMB_ERR_BAD_ARG;
-  Kv4Attn p{*d, out, q, lens, counts, pages, layer, n, heads / d->heads, 1, scale * 1.4426950408889634f, qb, qt, qh, ob, ot, oh, status};
-  return dtype == LLMB_BF16 ? run_type<__nv_bfloat16>(p, st) : run_type<float>(p, st);
+// The arguments of a call as the Python side (ops/kv4.py) packs them.
+struct Kv4AttendArgs {
+  void* out; const void* q; const int *lens, *counts, *pages;   // counts, pages: optional
+  int* status;
+  long long qb, qt, qh, ob, ot, oh;
+  float scale;
+  int layer, n, heads, dtype, pad;
+};
+
+LLMB_API int llmb_attention_kv4(const Kv4Desc* d, const Kv4AttendArgs* a, cudaStream_t st) {
+  if (a->heads % d->heads) return LLMB_ERR_BAD_ARG;
+  Kv4Attn p{*d, a->out, a->q, a->lens, a->counts, a->pages, a->layer, a->n, a->heads / d->heads, 1, a->scale * 1.4426950408889634f,
+            a->qb, a->qt, a->qh, a->ob, a->ot, a->oh, a->status};
+  return a->dtype == LLMB_BF16 ? run_type<__nv_bfloat16>(p, st) : run_type<float>(p, st);
 }

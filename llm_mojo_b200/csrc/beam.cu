@@ -200,20 +200,25 @@ __global__ void __launch_bounds__(THREADS) beam_merge_kernel(float* __restrict__
 }
 }  // namespace
 
-LLMB_API long long llmb_beam_select_work_bytes(int B, int K, int V) {
-  return (long long)B * K * ceil_div(V, CHUNK) * (8 + 8LL * K);
-}
+// The arguments of a call as the Python side (ops/beam.py) packs them.  work: B K chunks (8 + 8 K) bytes.
+struct BeamSelectArgs {
+  float* scores_out; int *tokens, *parents; bool* finished_out;          // finished_out: optional
+  const void* logits; const float* scores; const bool* finished;         // finished: optional
+  void* work;
+  long long ld;
+  int B, K, V, eos, dtype, pad;
+};
 
-LLMB_API int llmb_beam_select(float* scores_out, int* tokens, int* parents, bool* finished_out, const void* logits, const float* scores, const bool* finished,
-                              int B, int K, int V, long long ld, int eos, int dtype, void* work, cudaStream_t st) {
-  const int chunks = ceil_div(V, CHUNK), rows = B * K;
+LLMB_API int llmb_beam_select(const BeamSelectArgs* a, cudaStream_t st) {
+  const int K = a->K, V = a->V, chunks = ceil_div(V, CHUNK), rows = a->B * K;
   if (K < 1 || K > BEAM_MAX || rows > 65535 || (long long)K * chunks * 4 > 40 * 1024) return LLMB_ERR_BAD_ARG;
-  float2* stats = (float2*)work;
+  float2* stats = (float2*)a->work;
   unsigned long long* lists = (unsigned long long*)(stats + (long long)rows * chunks);
   const dim3 grid(chunks, rows);
-  int rc = dtype == LLMB_BF16 ? launch_pdl(beam_chunk_kernel<__nv_bfloat16>, grid, THREADS, 0, st, stats, lists, (const __nv_bfloat16*)logits, finished, K, V, ld, chunks)
-                              : launch_pdl(beam_chunk_kernel<float>, grid, THREADS, 0, st, stats, lists, (const float*)logits, finished, K, V, ld, chunks);
+  int rc = a->dtype == LLMB_BF16
+               ? launch_pdl(beam_chunk_kernel<__nv_bfloat16>, grid, THREADS, 0, st, stats, lists, (const __nv_bfloat16*)a->logits, a->finished, K, V, a->ld, chunks)
+               : launch_pdl(beam_chunk_kernel<float>, grid, THREADS, 0, st, stats, lists, (const float*)a->logits, a->finished, K, V, a->ld, chunks);
   if (rc) return rc;
-  return launch_pdl(beam_merge_kernel, B, THREADS, (size_t)K * chunks * 4, st, scores_out, tokens, parents, finished_out, scores, finished, (const float2*)stats,
-                    (const unsigned long long*)lists, K, V, eos, chunks);
+  return launch_pdl(beam_merge_kernel, a->B, THREADS, (size_t)K * chunks * 4, st, a->scores_out, a->tokens, a->parents, a->finished_out, a->scores, a->finished,
+                    (const float2*)stats, (const unsigned long long*)lists, K, V, a->eos, chunks);
 }

@@ -265,23 +265,32 @@ int values(const Kv4Desc& d, int layer, void* k, void* v, const int* start, cons
 }
 }  // namespace
 
-LLMB_API int llmb_kv4_append(const Kv4Desc* d, int layer, const void* k, const void* v, const int* start, const int* counts, int n,
-                             long long kb, long long kt, long long kh, long long vb, long long vt, long long vh, int dtype, cudaStream_t st) {
-  const RowStrides sk{kb, kt, kh}, sv{vb, vt, vh};
-  if (dtype == LLMB_BF16) { KV4_HEADS(d->head_size, (append<__nv_bfloat16, HD>(*d, layer, k, v, start, counts, n, sk, sv, st))) }
-  KV4_HEADS(d->head_size, (append<float, HD>(*d, layer, k, v, start, counts, n, sk, sv, st)))
+// The arguments of a call as the Python side (ops/kv4.py) packs them.
+struct Kv4AppendArgs {
+  const void *k, *v; const int *start, *counts;        // counts: optional
+  long long kb, kt, kh, vb, vt, vh;
+  int layer, n, dtype, pad;
+};
+struct Kv4ValuesArgs {
+  void *k, *v; const int *start, *pages;               // pages: optional
+  long long out_layer, kb, kt, kh, vb, vt, vh;         // layer -1: all layers, out_layer elements apart
+  int layer, n, dtype, pad;
+};
+
+LLMB_API int llmb_kv4_append(const Kv4Desc* d, const Kv4AppendArgs* a, cudaStream_t st) {
+  const RowStrides sk{a->kb, a->kt, a->kh}, sv{a->vb, a->vt, a->vh};
+  if (a->dtype == LLMB_BF16) { KV4_HEADS(d->head_size, (append<__nv_bfloat16, HD>(*d, a->layer, a->k, a->v, a->start, a->counts, a->n, sk, sv, st))) }
+  KV4_HEADS(d->head_size, (append<float, HD>(*d, a->layer, a->k, a->v, a->start, a->counts, a->n, sk, sv, st)))
 }
 
-// layer -1: all layers, out_layer elements apart
-LLMB_API int llmb_kv4_values(const Kv4Desc* d, int layer, void* k, void* v, const int* start, const int* pages, int n, long long out_layer,
-                             long long kb, long long kt, long long kh, long long vb, long long vt, long long vh, int dtype, cudaStream_t st) {
-  const RowStrides sk{kb, kt, kh}, sv{vb, vt, vh};
-  if (dtype == LLMB_BF16) { KV4_HEADS(d->head_size, (values<__nv_bfloat16, HD>(*d, layer, k, v, start, pages, n, out_layer, sk, sv, st))) }
-  KV4_HEADS(d->head_size, (values<float, HD>(*d, layer, k, v, start, pages, n, out_layer, sk, sv, st)))
+LLMB_API int llmb_kv4_values(const Kv4Desc* d, const Kv4ValuesArgs* a, cudaStream_t st) {
+  const RowStrides sk{a->kb, a->kt, a->kh}, sv{a->vb, a->vt, a->vh};
+  if (a->dtype == LLMB_BF16) { KV4_HEADS(d->head_size, (values<__nv_bfloat16, HD>(*d, a->layer, a->k, a->v, a->start, a->pages, a->n, a->out_layer, sk, sv, st))) }
+  KV4_HEADS(d->head_size, (values<float, HD>(*d, a->layer, a->k, a->v, a->start, a->pages, a->n, a->out_layer, sk, sv, st)))
 }
 
 LLMB_API int llmb_kv4_reorder(const Kv4Desc* d, int* pages, int* lens, const int* parents, int K, cudaStream_t st) {
-  const int items = d->slots / K;
+  const int items = K > 0 ? d->slots / K : 0;
   if (K < 1 || K > 64 || d->layers > 65535 || d->heads > 65535) return LLMB_ERR_BAD_ARG;
   int rc = launch_pdl(kv4_reorder_kernel, dim3(items, d->heads, d->layers), REORDER_THREADS, 0, st, *d, (const int*)lens, parents, K);
   if (rc) return rc;

@@ -85,12 +85,11 @@ _SIGS = {
     "llmb_attention_bwd_fused": [c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_int, c_int, c_int, c_p, c_p],
     "llmb_attention_bwd_fused_stats_floats": [c_int, c_int, c_int],
     "llmb_attention_bwd_fused_acc_floats": [c_int, c_int, c_int],
-    "llmb_kv4_append": [c_p, c_int, c_p, c_p, c_p, c_p, c_int, c_ll, c_ll, c_ll, c_ll, c_ll, c_ll, c_int, c_p],
-    "llmb_kv4_values": [c_p, c_int, c_p, c_p, c_p, c_p, c_int, c_ll, c_ll, c_ll, c_ll, c_ll, c_ll, c_ll, c_int, c_p],
+    "llmb_kv4_append": [c_p, c_p, c_p],
+    "llmb_kv4_values": [c_p, c_p, c_p],
     "llmb_kv4_reorder": [c_p, c_p, c_p, c_p, c_int, c_p],
-    "llmb_attention_kv4": [c_p, c_int, c_p, c_p, c_p, c_p, c_p, c_int, c_int, c_f, c_ll, c_ll, c_ll, c_ll, c_ll, c_ll, c_int, c_p, c_p],
-    "llmb_beam_select_work_bytes": [c_int, c_int, c_int],
-    "llmb_beam_select": [c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_int, c_int, c_int, c_ll, c_int, c_int, c_p, c_p],
+    "llmb_attention_kv4": [c_p, c_p, c_p],
+    "llmb_beam_select": [c_p, c_p],
     "llmb_loss_accumulate": [c_p, c_p, c_int, c_f, c_p],
     "llmb_gpt2_step_bytes": [],
     "llmb_gpt2_lowp_scratch_bytes": [c_p],
@@ -99,8 +98,7 @@ _SIGS = {
     "llmb_gpt2_backward": [c_p, c_p],
 }
 _RET_LL = {"llmb_encoder_bwd_scratch_bytes", "llmb_dbias_scratch_bytes", "llmb_layernorm_bwd_scratch_bytes",
-           "llmb_nvfp4_scale_bytes", "llmb_gpt2_lowp_scratch_bytes", "llmb_gpt2_lowp_kept_bytes", "llmb_attention_bwd_fused_stats_floats", "llmb_attention_bwd_fused_acc_floats",
-           "llmb_beam_select_work_bytes"}
+           "llmb_nvfp4_scale_bytes", "llmb_gpt2_lowp_scratch_bytes", "llmb_gpt2_lowp_kept_bytes", "llmb_attention_bwd_fused_stats_floats", "llmb_attention_bwd_fused_acc_floats"}
 
 
 def lib_path() -> str:

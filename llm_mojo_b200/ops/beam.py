@@ -1,14 +1,17 @@
 """Beam search: the selection over beams and vocabulary (``csrc/beam.cu``; the cache follows with ``ops.kv4_reorder``)."""
 from __future__ import annotations
 
+import struct
 from typing import Optional
 
 import torch
 
-from ._lib import check, dtype_code, lib, ptr
-from .kv4 import _count, _ints, _on
+from . import _count
+from ._lib import lib
+from .kv4 import _call, _ints
 
 BEAM_MAX = 64
+_SELECT = struct.Struct("@8Pq6i")            # BeamSelectArgs of csrc/beam.cu
 
 
 def beam_select(scores_out: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, logits: torch.Tensor, scores: torch.Tensor,
@@ -25,44 +28,56 @@ def beam_select(scores_out: torch.Tensor, tokens: torch.Tensor, parents: torch.T
     log-sum-exp (a NaN or +inf among them, or nothing but -inf), offers -inf throughout.  Outputs may not share memory with inputs.
 
     The order within a beam is that of its logits, between beams that of the sums in 64 bits, with each log-sum-exp from fp32 exponentials."""
-    if scores.dim() != 2 or scores.dtype != torch.float32 or not scores.is_contiguous():
-        raise ValueError(f"scores must be a contiguous fp32 [B, K], not {scores.dtype} {tuple(scores.shape)}")
-    B, K = scores.shape
-    dev = scores.device
-    if logits.dim() != 2 or logits.shape[0] != B * K or logits.device != dev or (logits.numel() and logits.stride(1) != 1):
-        raise ValueError(f"logits must be [{B * K}, at least {vocab_size}] on {dev} with dense rows, not {tuple(logits.shape)} on {logits.device}")
-    if logits.dtype not in (torch.bfloat16, torch.float32):
-        raise TypeError(f"logits must be bf16 or fp32, not {logits.dtype}")
+    shape, dev = scores.shape, scores.device
+    if len(shape) != 2 or scores.dtype is not torch.float32 or not scores.is_contiguous():
+        raise ValueError(f"scores must be a contiguous fp32 [B, K], not {scores.dtype} {tuple(shape)}")
+    B, K = shape
+    rows, dtype = logits.shape, logits.dtype
+    if len(rows) != 2 or rows[0] != B * K or logits.device != dev or (logits.stride(1) != 1 and logits.numel()):
+        raise ValueError(f"logits must be [{B * K}, at least {vocab_size}] on {dev} with dense rows, not {tuple(rows)} on {logits.device}")
+    if dtype is not torch.bfloat16 and dtype is not torch.float32:
+        raise TypeError(f"logits must be bf16 or fp32, not {dtype}")
     if not 1 <= K <= BEAM_MAX:
         raise ValueError(f"1 to {BEAM_MAX} beams, not {K}")
-    if not K <= vocab_size <= logits.shape[1] or K * vocab_size >= 2 ** 31:
-        raise ValueError(f"vocabulary of {vocab_size}: at least {K} beams, at most the {logits.shape[1]} columns, and K x V below 2^31")
+    if not K <= vocab_size <= rows[1] or K * vocab_size >= 2 ** 31:
+        raise ValueError(f"vocabulary of {vocab_size}: at least {K} beams, at most the {rows[1]} columns, and K x V below 2^31")
     if B * K > 65535 or K * -(-vocab_size // 4096) > 10240:
         raise ValueError(f"{B} items of {K} beams over {vocab_size} tokens are too many: at most 65535 rows, and K x V up to 40 million")
     if not -1 <= eos < vocab_size:
         raise ValueError(f"eos {eos} is no token of a vocabulary of {vocab_size}")
     if finished is not None and eos < 0:
         raise ValueError("finished beams go on with eos: it is needed")
-    if scores_out.dtype != torch.float32 or tuple(scores_out.shape) != (B, K) or scores_out.device != dev or not scores_out.is_contiguous():
-        raise ValueError(f"scores_out must be a contiguous fp32 {(B, K)} on {dev}")
-    _ints(tokens, "tokens", (B, K), dev)
-    _ints(parents, "parents", (B, K), dev)
+    if scores_out.dtype is not torch.float32 or scores_out.shape != shape or scores_out.device != dev or not scores_out.is_contiguous():
+        raise ValueError(f"scores_out must be a contiguous fp32 {tuple(shape)} on {dev}")
+    so, si = scores_out.data_ptr(), scores.data_ptr()
+    tk, pa = _ints(tokens, "tokens", shape, dev), _ints(parents, "parents", shape, dev)
+    if tokens is None or parents is None:
+        raise ValueError("tokens and parents are outputs that every call needs")
+    n = B * K
+    spans = [(so, 4 * n), (tk, 4 * n), (pa, 4 * n), (si, 4 * n)]
+    fi = fo = 0
     for name, t in (("finished", finished), ("finished_out", finished_out)):
-        if t is not None and (t.dtype != torch.bool or tuple(t.shape) != (B, K) or t.device != dev or not t.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous bool {(B, K)} on {dev}")
-    outs = [t for t in (scores_out, tokens, parents, finished_out) if t is not None]
-    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (*outs, scores, *([finished] if finished is not None else []))]
-    if B and any(a[0] < b[1] and b[0] < a[1] for i, a in enumerate(spans[:len(outs)]) for b in spans[i + 1:]):
-        raise ValueError("outputs must not share memory with each other or with inputs")
-    if B == 0:
+        if t is None:
+            continue
+        if t.dtype is not torch.bool or t.shape != shape or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous bool {tuple(shape)} on {dev}")
+        at = t.data_ptr()
+        spans.append((at, n))
+        fi, fo = (at, fo) if t is finished else (fi, at)
+    if n == 0:
         return
+    spans.sort()
+    end = 0
+    for at, size in spans:
+        if at < end:
+            raise ValueError("outputs must not share memory with each other or with inputs")
+        end = at + size
     if scores.is_cuda:
         L = lib()
-        with _on(dev) as stream:
-            # one call's own workspace: it lives as long as the work on this stream, and captured graphs do not share it
-            work = torch.empty(L.llmb_beam_select_work_bytes(B, K, vocab_size), dtype=torch.uint8, device=dev)
-            check(L.llmb_beam_select(ptr(scores_out), ptr(tokens), ptr(parents), ptr(finished_out), ptr(logits), ptr(scores), ptr(finished),
-                                     B, K, vocab_size, logits.stride(0), eos, dtype_code(logits), ptr(work), stream), "beam_select")
+        # one call's own workspace: it lives as long as the work on this stream, and captured graphs do not share it
+        work = torch.empty(n * -(-vocab_size // 4096) * (8 + 8 * K), dtype=torch.uint8, device=dev)
+        _call(L.llmb_beam_select, "beam_select", dev,
+              _SELECT.pack(so, tk, pa, fo, logits.data_ptr(), si, fi, work.data_ptr(), logits.stride(0), B, K, vocab_size, eos, 1 if dtype is torch.bfloat16 else 0, 0))
         _count(2)
         return
     x = logits[:, :vocab_size].double().view(B, K, vocab_size)

@@ -15,14 +15,14 @@ CUDA tensors run ``csrc/kv4.cu`` and ``csrc/attention_kv4.cu``; CPU tensors run 
 """
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 from typing import Optional
 
 import torch
 
-from . import _lib
-from ._lib import check, dtype_code, lib, ptr, status_word
+from . import _count
+from ._lib import check, lib, status_word
 
 KV4_PAGE = 64
 KV4_UNIT = 2.0 ** -4          # largest value 2688 / 16 = 168; scales of 2^-6 and more (values of 0.006 and more) have all their bits
@@ -30,13 +30,11 @@ KV4_HEAD_SIZES = (32, 64, 80, 96, 128)
 _LEVELS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
 
-class _Kv4Desc(ctypes.Structure):
-    """``Kv4Desc`` of ``csrc/kv4.cuh``."""
-    _fields_ = [("kc", ctypes.c_void_p), ("ks", ctypes.c_void_p), ("vc", ctypes.c_void_p), ("vs", ctypes.c_void_p),
-                ("code_layer", ctypes.c_longlong), ("code_slot", ctypes.c_longlong),
-                ("scale_layer", ctypes.c_longlong), ("scale_slot", ctypes.c_longlong),
-                ("layers", ctypes.c_int), ("slots", ctypes.c_int), ("heads", ctypes.c_int), ("capacity", ctypes.c_int),
-                ("head_size", ctypes.c_int), ("k_exp", ctypes.c_int), ("v_exp", ctypes.c_int), ("pad", ctypes.c_int)]
+# Arguments travel as packed structures, one pointer a call: a ctypes call that converts twenty arguments takes longer than a launch.
+_DESC = struct.Struct("@4P4q8i")             # Kv4Desc of csrc/kv4.cuh
+_APPEND = struct.Struct("@4P6q4i")           # Kv4AppendArgs of csrc/kv4.cu
+_VALUES = struct.Struct("@4P7q4i")           # Kv4ValuesArgs
+_ATTEND = struct.Struct("@6P6qf5i")          # Kv4AttendArgs of csrc/attention_kv4.cu
 
 
 def _exponent(unit: float, name: str) -> int:
@@ -51,7 +49,7 @@ class KV4Cache:
     slot, some of the layers); heads, tokens and values lie densely, every row 16-byte aligned."""
 
     __slots__ = ("k_codes", "k_scales", "v_codes", "v_scales", "k_unit", "v_unit", "layers", "slots", "kv_heads", "capacity", "head_size",
-                 "device", "_desc", "_ref")
+                 "device", "_desc")
 
     def __init__(self, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor,
                  k_unit: float = KV4_UNIT, v_unit: float = KV4_UNIT):
@@ -60,31 +58,30 @@ class KV4Cache:
         L, S, H, T, half = k_codes.shape
         if 2 * half not in KV4_HEAD_SIZES:
             raise ValueError(f"head size {2 * half}: the cache takes {KV4_HEAD_SIZES}")
-        if T % KV4_PAGE or T == 0 or min(L, S, H) == 0:
+        if T % KV4_PAGE or T == 0 or L == 0 or S == 0 or H == 0:
             raise ValueError(f"capacity {T} must be a multiple of {KV4_PAGE}, and no dimension of {tuple(k_codes.shape)} empty")
-        if H > 65535 or S > 65535:
-            raise ValueError(f"at most 65535 slots and heads, not {S} and {H}")
-        codes, scales = (L, S, H, T, half), (L, S, H, T, half // 8)
+        if H > 65535 or S > 65535 or L > 65535:
+            raise ValueError(f"at most 65535 layers, slots and heads, not {L}, {S} and {H}")
         dev = k_codes.device
         cs, ss = k_codes.stride(), k_scales.stride()
-        for name, t, shape, strides in (("k_codes", k_codes, codes, cs), ("k_scales", k_scales, scales, ss),
-                                        ("v_codes", v_codes, codes, cs), ("v_scales", v_scales, scales, ss)):
-            if t.dtype != torch.uint8 or tuple(t.shape) != shape or t.device != dev:
+        p = (k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr())
+        codes, scales = (L, S, H, T, half), (L, S, H, T, half // 8)
+        for name, t, shape, st, at in (("k_codes", k_codes, codes, cs, p[0]), ("k_scales", k_scales, scales, ss, p[1]),
+                                       ("v_codes", v_codes, codes, cs, p[2]), ("v_scales", v_scales, scales, ss, p[3])):
+            if t.dtype is not torch.uint8 or t.shape != shape or t.device != dev:
                 raise ValueError(f"{name} must be uint8 {shape} on {dev}, not {t.dtype} {tuple(t.shape)} on {t.device}")
+            if t.stride() != st:
+                raise ValueError(f"{name}: keys and values must have the same strides, not {t.stride()} and {st}")
             c = shape[4]
-            st = t.stride()
-            if st != strides:
-                raise ValueError(f"{name}: keys and values must have the same strides, not {st} and {strides}")
-            if st[4] != 1 or st[3] != c or (H > 1 and st[2] != T * c) or (t.data_ptr() | (st[1] if S > 1 else 0) | (st[0] if L > 1 else 0)) % 16:
+            if st[4] != 1 or st[3] != c or (H > 1 and st[2] != T * c) or (at | (st[1] if S > 1 else 0) | (st[0] if L > 1 else 0)) % 16:
                 raise ValueError(f"{name}: heads, tokens and values must lie densely, slots and layers 16-byte aligned (strides {st})")
-            if (S > 1 and st[1] < H * T * c) or (L > 1 and st[0] < H * T * c):
+            row = H * T * c
+            if (S > 1 and st[1] < row) or (L > 1 and st[0] < row) or (L > 1 and S > 1 and (S - 1) * st[1] + row > st[0] and (L - 1) * st[0] + row > st[1]):
                 raise ValueError(f"{name}: slots and layers must not overlap (strides {st})")
         self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
         self.k_unit, self.v_unit = k_unit, v_unit
         self.layers, self.slots, self.kv_heads, self.capacity, self.head_size, self.device = L, S, H, T, 2 * half, dev
-        self._desc = _Kv4Desc(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), cs[0], cs[1], ss[0], ss[1],
-                              L, S, H, T, 2 * half, _exponent(k_unit, "k_unit"), _exponent(v_unit, "v_unit"), 0)
-        self._ref = ctypes.addressof(self._desc)
+        self._desc = _DESC.pack(*p, cs[0], cs[1], ss[0], ss[1], L, S, H, T, 2 * half, _exponent(k_unit, "k_unit"), _exponent(v_unit, "v_unit"), 0)
 
     @classmethod
     def empty(cls, layers: int, slots: int, kv_heads: int, max_len: int, head_size: int, device="cuda", k_unit: float = KV4_UNIT,
@@ -109,55 +106,55 @@ class KV4Cache:
 
 
 # ------------------------------------------------------------------ arguments
-class _on:
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    lambda index: torch.cuda.current_stream(index).cuda_stream
+
+
+def _call(fn, name: str, device: torch.device, *args) -> None:
     """Launches go to the current stream of the tensors' device, whichever device is current."""
-    __slots__ = ("guard", "stream")
-
-    def __init__(self, device: torch.device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self) -> int:
-        if self.guard is not None:
-            self.guard.__enter__()
-        return _lib.stream()
-
-    def __exit__(self, *e):
-        if self.guard is not None:
-            self.guard.__exit__(*e)
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        check(rc, name)
 
 
-def _ints(t: Optional[torch.Tensor], name: str, shape: tuple, device) -> None:
+def _ints(t: Optional[torch.Tensor], name: str, shape: tuple, device) -> int:
+    """The address of an optional tensor of integers."""
     if t is None:
-        return
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
+        return 0
+    if t.dtype is not torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 {shape} on {device}, not {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
 
 
-def _layer(cache: KV4Cache, layer: int) -> int:
+def _layer(cache: KV4Cache, layer: int) -> None:
     if not isinstance(layer, int) or not 0 <= layer < cache.layers:
         raise ValueError(f"layer {layer!r} of a cache of {cache.layers} layers")
-    return layer
 
 
-def _rows(t: torch.Tensor, name: str, shape: tuple, dtype, device) -> None:
-    if t.dtype != dtype or tuple(t.shape) != shape or t.device != device:
-        raise ValueError(f"{name} must be {dtype} {shape} on {device}, not {t.dtype} {tuple(t.shape)} on {t.device}")
-    if t.numel() and t.stride(-1) != 1:
-        raise ValueError(f"{name}: the values of a head must lie densely (strides {t.stride()})")
+def _rows(t: torch.Tensor, name: str, shape: tuple, dtype, device) -> tuple:
+    """The strides of a tensor of rows."""
+    if t.dtype is not dtype or t.shape != shape or t.device != device:
+        raise ValueError(f"{name} must be {dtype} {tuple(shape)} on {device}, not {t.dtype} {tuple(t.shape)} on {t.device}")
+    st = t.stride()
+    if st[-1] != 1 and t.numel():
+        raise ValueError(f"{name}: the values of a head must lie densely (strides {st})")
+    return st
 
 
 def _spread(t: torch.Tensor, name: str) -> None:
     """An output whose elements share memory would be written by several threads."""
+    if t.is_contiguous():
+        return
     span = 1
     for n, s in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n > 1), key=lambda p: p[1]):
         if s < span:
             raise ValueError(f"{name}: elements of an output must not overlap (shape {tuple(t.shape)}, strides {t.stride()})")
-        span = s * n
-
-
-def _count(n: int = 1) -> None:
-    from .. import ops
-    ops._count(n)
+        span += s * (n - 1)
 
 
 # ------------------------------------------------------------------ the definitions, on any device, in fp32
@@ -187,23 +184,21 @@ def kv4_append(cache: KV4Cache, layer: int, k: torch.Tensor, v: torch.Tensor, st
 
     A value beyond the largest one (2688 units) becomes that one.  A token and head with a non-finite key or value has no 4-bit form: its
     key and its value are kept as NaN, and every query that sees it answers NaN."""
-    S, n, H, hd = k.shape if k.dim() == 4 else (None,) * 4
-    if (S, H, hd) != (cache.slots, cache.kv_heads, cache.head_size):
-        raise ValueError(f"k must be [{cache.slots}, n, {cache.kv_heads}, {cache.head_size}], not {tuple(k.shape)}")
-    if k.dtype not in (torch.bfloat16, torch.float32):
-        raise TypeError(f"k and v must be bf16 or fp32, not {k.dtype}")
+    shape = k.shape
+    if len(shape) != 4 or shape[0] != cache.slots or shape[2] != cache.kv_heads or shape[3] != cache.head_size:
+        raise ValueError(f"k must be [{cache.slots}, n, {cache.kv_heads}, {cache.head_size}], not {tuple(shape)}")
+    S, n, H, hd = shape
+    dtype, dev = k.dtype, cache.device
+    if dtype is not torch.bfloat16 and dtype is not torch.float32:
+        raise TypeError(f"k and v must be bf16 or fp32, not {dtype}")
     _layer(cache, layer)
-    _rows(k, "k", (S, n, H, hd), k.dtype, cache.device)
-    _rows(v, "v", (S, n, H, hd), k.dtype, cache.device)
-    _ints(start, "start", (S,), cache.device)
-    _ints(counts, "counts", (S,), cache.device)
+    ks, vs = _rows(k, "k", shape, dtype, dev), _rows(v, "v", shape, dtype, dev)
+    at, cnt = _ints(start, "start", (S,), dev), _ints(counts, "counts", (S,), dev)
     if n == 0:
         return
     if k.is_cuda:
-        ks, vs = k.stride(), v.stride()
-        with _on(cache.device) as stream:
-            check(lib().llmb_kv4_append(cache._ref, layer, ptr(k), ptr(v), ptr(start), ptr(counts), n, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-                                        dtype_code(k), stream), "kv4_append")
+        _call(lib().llmb_kv4_append, "kv4_append", dev, cache._desc,
+              _APPEND.pack(k.data_ptr(), v.data_ptr(), at, cnt, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], layer, n, 1 if dtype is torch.bfloat16 else 0, 0))
         _count()
         return
     kf, vf = k.float(), v.float()
@@ -225,27 +220,27 @@ def kv4_values(k_out: torch.Tensor, v_out: torch.Tensor, cache: KV4Cache, layer:
     """Reads back what the cache holds: ``k_out``, ``v_out`` [slots, n, kv_heads, head_size] (bf16, in which every value is exact, or fp32) of
     the positions ``start[s] + i`` of one layer, or [layers, slots, ...] of all layers (``layer`` None).  Positions outside the cache read as
     zeros, pages whose entry in ``pages`` names no slot as NaN."""
-    lead = (cache.layers, cache.slots) if layer is None else (cache.slots,)
-    n = k_out.shape[-3] if k_out.dim() == len(lead) + 3 else -1
-    shape = (*lead, n, cache.kv_heads, cache.head_size)
-    if k_out.dtype not in (torch.bfloat16, torch.float32):
-        raise TypeError(f"k_out and v_out must be bf16 or fp32, not {k_out.dtype}")
+    dtype, dev, shape = k_out.dtype, cache.device, k_out.shape
+    lead = (cache.slots,) if layer is not None else (cache.layers, cache.slots)
+    if len(shape) != len(lead) + 3 or shape[:-3] != lead or shape[-2] != cache.kv_heads or shape[-1] != cache.head_size:
+        raise ValueError(f"k_out must be {[*lead, 'n', cache.kv_heads, cache.head_size]}, not {tuple(shape)}")
+    n = shape[-3]
+    if dtype is not torch.bfloat16 and dtype is not torch.float32:
+        raise TypeError(f"k_out and v_out must be bf16 or fp32, not {dtype}")
     if layer is not None:
         _layer(cache, layer)
-    for name, t in (("k_out", k_out), ("v_out", v_out)):
-        _rows(t, name, shape, k_out.dtype, cache.device)
-        _spread(t, name)
-        if layer is None and t.numel() and t.stride() != k_out.stride():
-            raise ValueError(f"k_out and v_out must have the same strides, not {k_out.stride()} and {t.stride()}")
-    _ints(start, "start", (cache.slots,), cache.device)
-    _ints(pages, "pages", (cache.slots, cache.capacity // KV4_PAGE), cache.device)
+    ks, vs = _rows(k_out, "k_out", shape, dtype, dev), _rows(v_out, "v_out", shape, dtype, dev)
+    _spread(k_out, "k_out")
+    _spread(v_out, "v_out")
+    if layer is None and n and ks != vs:
+        raise ValueError(f"k_out and v_out must have the same strides, not {ks} and {vs}")
+    at, pg = _ints(start, "start", (cache.slots,), dev), _ints(pages, "pages", (cache.slots, cache.capacity // KV4_PAGE), dev)
     if n == 0:
         return
     if k_out.is_cuda:
-        ks, vs = k_out.stride(), v_out.stride()
-        with _on(cache.device) as stream:
-            check(lib().llmb_kv4_values(cache._ref, -1 if layer is None else layer, ptr(k_out), ptr(v_out), ptr(start), ptr(pages), n,
-                                        ks[0] if layer is None else 0, *ks[-4:-1], *vs[-4:-1], dtype_code(k_out), stream), "kv4_values")
+        _call(lib().llmb_kv4_values, "kv4_values", dev, cache._desc,
+              _VALUES.pack(k_out.data_ptr(), v_out.data_ptr(), at, pg, ks[0] if layer is None else 0, ks[-4], ks[-3], ks[-2], vs[-4], vs[-3], vs[-2],
+                           -1 if layer is None else layer, n, 1 if dtype is torch.bfloat16 else 0, 0))
         _count()
         return
     T, i = cache.capacity, torch.arange(n)
@@ -275,31 +270,28 @@ def attention_kv4(out: torch.Tensor, q: torch.Tensor, cache: KV4Cache, layer: in
     ``out`` may be ``q`` itself.  A page whose entry in ``pages`` names no slot gives NaN to every row that sees it.
 
     Scores, statistics and sums are in fp32.  lens above the capacity count as the capacity."""
-    if q.dim() != 4 or (q.shape[0], q.shape[3]) != (cache.slots, cache.head_size) or q.shape[2] % cache.kv_heads or q.shape[2] == 0:
-        raise ValueError(f"q must be [{cache.slots}, n, a multiple of {cache.kv_heads}, {cache.head_size}], not {tuple(q.shape)}")
-    if q.dtype not in (torch.bfloat16, torch.float32):
-        raise TypeError(f"q must be bf16 or fp32, not {q.dtype}")
-    S, n, heads, hd = q.shape
+    shape, dtype, dev = q.shape, q.dtype, cache.device
+    if len(shape) != 4 or shape[0] != cache.slots or shape[3] != cache.head_size or shape[2] % cache.kv_heads or shape[2] == 0:
+        raise ValueError(f"q must be [{cache.slots}, n, a multiple of {cache.kv_heads}, {cache.head_size}], not {tuple(shape)}")
+    if dtype is not torch.bfloat16 and dtype is not torch.float32:
+        raise TypeError(f"q must be bf16 or fp32, not {dtype}")
+    S, n, heads, hd = shape
     _layer(cache, layer)
-    _rows(q, "q", (S, n, heads, hd), q.dtype, cache.device)
-    _rows(out, "out", (S, n, heads, hd), q.dtype, cache.device)
+    qs, os_ = _rows(q, "q", shape, dtype, dev), _rows(out, "out", shape, dtype, dev)
     _spread(out, "out")
-    _ints(lens, "lens", (S,), cache.device)
-    _ints(counts, "counts", (S,), cache.device)
-    _ints(pages, "pages", (S, cache.capacity // KV4_PAGE), cache.device)
-    scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
+    ln, cnt = _ints(lens, "lens", (S,), dev), _ints(counts, "counts", (S,), dev)
+    pg = _ints(pages, "pages", (S, cache.capacity // KV4_PAGE), dev)
+    scale = hd ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError(f"scale must be finite, not {scale}")
-    if n * (heads // cache.kv_heads) > 2 ** 30:
+    if n * heads > 2 ** 30:
         raise ValueError(f"{n} rows of {heads} heads are too many")
     if n == 0:
         return
     if q.is_cuda:
-        qs, os_ = q.stride(), out.stride()
-        with _on(cache.device) as stream:
-            check(lib().llmb_attention_kv4(cache._ref, layer, ptr(out), ptr(q), ptr(lens), ptr(counts), ptr(pages), n, heads, scale,
-                                           qs[0], qs[1], qs[2], os_[0], os_[1], os_[2], dtype_code(q), ptr(status_word(cache.device)), stream),
-                  "attention_kv4")
+        _call(lib().llmb_attention_kv4, "attention_kv4", dev, cache._desc,
+              _ATTEND.pack(out.data_ptr(), q.data_ptr(), ln, cnt, pg, status_word(dev).data_ptr(), qs[0], qs[1], qs[2], os_[0], os_[1], os_[2], scale, layer, n,
+                           heads, 1 if dtype is torch.bfloat16 else 0, 0))
         _count()
         return
     group, T = heads // cache.kv_heads, cache.capacity
@@ -338,14 +330,13 @@ def kv4_reorder(cache: KV4Cache, pages: torch.Tensor, lens: torch.Tensor, parent
     B, K = parents.shape
     if K > 64:
         raise ValueError(f"at most 64 beams, not {K}")
-    _ints(parents, "parents", (B, K), cache.device)
-    _ints(lens, "lens", (cache.slots,), cache.device)
-    _ints(pages, "pages", (cache.slots, cache.capacity // KV4_PAGE), cache.device)
+    dev = cache.device
     if pages is None or lens is None:
         raise ValueError("kv4_reorder permutes pages and lens: both are needed")
+    par, ln = _ints(parents, "parents", (B, K), dev), _ints(lens, "lens", (cache.slots,), dev)
+    pg = _ints(pages, "pages", (cache.slots, cache.capacity // KV4_PAGE), dev)
     if lens.is_cuda:
-        with _on(cache.device) as stream:
-            check(lib().llmb_kv4_reorder(cache._ref, ptr(pages), ptr(lens), ptr(parents), K, stream), "kv4_reorder")
+        _call(lib().llmb_kv4_reorder, "kv4_reorder", dev, cache._desc, pg, ln, par, K)
         _count(2)
         return
     slot = torch.arange(cache.slots)

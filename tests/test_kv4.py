@@ -107,6 +107,10 @@ def test_cache_refusals():
     with pytest.raises(ValueError, match="layers"):
         ops.KV4Cache(*(x[0] for x in t))
     assert c.select(slice(0, None, 2)).slots == 1
+    assert _cache(layers=2, slots=6).select(slice(0, None, 4)).slots == 2
+    with pytest.raises(ValueError, match="overlap"):
+        ops.KV4Cache(*(x.as_strided((2, 2, *x.shape[2:]), (x.stride(1) * 3 // 2 // 16 * 16, x.stride(1), *x.stride()[2:]))
+                       for x in (lambda y: (y.k_codes, y.k_scales, y.v_codes, y.v_scales))(_cache(slots=4))))
 
 
 def test_append_and_values_refusals():
