@@ -20,27 +20,32 @@ struct Kv4Attn {
   float scale_log2;
   long long qb, qt, qh, ob, ot, oh;                    // element strides
   int* status;
+  bool q_vec;                                          // rows of q can be read 16 bytes at a time
 };
 
-// The form on the tensor core, for bf16 and fp32.  The products are taken transposed, S^T = K q^T and o^T = V^T P^T (mma.sync m16n8k16, f16
-// operands, fp32 sums): 16 keys fill a tile's rows and eight columns are rows of q, so that a single query pads to 8 and not to 128
-// (as it would in a tcgen05 product), and the codes go from shared memory to registers straight into operands:
+// The products are taken transposed, S^T = K q^T and o^T = V^T P^T (mma.sync m16n8k16, f16 operands, fp32 sums): 16 keys fill a tile's rows
+// and eight columns are rows of q, so that a single query pads to 8 and not to 128 (as it would in a tcgen05 product), and the codes
+// go from shared memory to registers straight into operands:
 //   K  a lane holds contiguous words of a key's row; the order of the contraction index is free as long as q is laid out alike;
-//   V  a lane holds one word (eight columns) of four keys; cvt gives pairs of columns, two byte permutations pairs of keys.
+//   V  a lane holds one word (eight columns) of four keys.  cvt turns a byte into a pair of columns of one key, but the contraction runs over
+//      keys.  With few rows (NARROW: two columns of the tile per row) the pair is contracted as it stands, against (p, 0) in a row's
+//      first column, which gives the even columns of o, and (0, p) in its second, the odd ones; with more rows two byte permutations
+//      of every four values make pairs of keys.
 // code x scale is exact in f16.  q is brought into f16's range by a power of two per row (exact for bf16; an fp32 row takes two columns, its
 // upper and its lower 11 bits), P is scaled by 2^15 (the rest of f16's range) and, for fp32, split alike.  P^T comes out of the accumulators of
 // S^T as the second product's other operand by a transposition within the warp (movmatrix).
 //
-// Each warp has a ring of its own of four key tiles, filled by untiled bulk copies (a tile is contiguous in each of the four tensors), and
+// Each warp has a ring of its own of key tiles, filled by untiled bulk copies (a tile is contiguous in each of the four tensors), and
 // runs its softmax with nobody to wait for; W warps (and a cluster's `splits` blocks) share a unit, one (slot, key head, rows).
-constexpr int MW = 4, NSTG = 4;
-template <typename T, int HD, int NT> struct MmaShape {
+constexpr int NSTG = 2, MOST_WARPS = 8, MOST_SPLITS = 16;
+template <typename T, int HD, int NT, bool NARROW> struct MmaShape {
   static constexpr int WORDS = HD / 8, NB = HD / BLOCK, WPT = (WORDS + 3) / 4, NWV = (WORDS + 7) / 8;
   static constexpr int TK = HD <= 64 ? 64 : 32, KS = NT == 1 ? TK : 32;         // keys of a tile; of one step of the softmax
-  static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1, ROWS = 8 * NT / PARTS;   // columns per row; rows of a unit
+  static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1, PER_ROW = PARTS * (NARROW ? 2 : 1), ROWS = 8 * NT / PER_ROW;   // columns per row; rows of a unit
   static constexpr int CODE_BYTES = TK * HD / 2, SCALE_BYTES = TK * NB, STAGE = 2 * (CODE_BYTES + SCALE_BYTES);
   static constexpr int WARP_BYTES = NSTG * STAGE;
-  static constexpr int SMEM = MW * WARP_BYTES + MW * NSTG * 8;
+  static constexpr int SMEM_WARP = WARP_BYTES + NSTG * 8;
+  static constexpr int WARPS_SM = NT > 2 || (NT == 2 && HD > 64) ? 8 : NT == 2 ? 12 : HD <= 64 ? 24 : 16;             // registers decide
   static_assert(ROWS * (HD + 2) * 4 <= WARP_BYTES && STAGE % 16 == 0 && SCALE_BYTES % 16 == 0, "");
 };
 
@@ -59,19 +64,24 @@ __device__ __forceinline__ void unpack8(uint32_t w, uint32_t (&h)[4]) {
       "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}" : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
 }
 __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) { uint32_t d; asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b)); return d; }
+__device__ __forceinline__ uint32_t low2(uint32_t a) { uint32_t d; asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tmov.b32 %0, {l, l};\n\t}" : "=r"(d) : "r"(a)); return d; }
+__device__ __forceinline__ uint32_t high2(uint32_t a) { uint32_t d; asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tmov.b32 %0, {h, h};\n\t}" : "=r"(d) : "r"(a)); return d; }
 __device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) { uint32_t d; asm("min.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b)); return d; }
 __device__ __forceinline__ uint32_t f16x2(float lo, float hi) { uint32_t d; asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo)); return d; }
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 constexpr float P_SHIFT = 15.f;                        // P <= 2^15
 
-template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(MW * 32) attention_kv4_mma_kernel(const Kv4Attn p, int log_w, int tiles) {
-  using S = MmaShape<T, HD, NT>;
-  constexpr int WPT = S::WPT, NWV = S::NWV, NB = S::NB, TK = S::TK, KS = S::KS, ROWS = S::ROWS, PARTS = S::PARTS, G16 = KS / 16;
-  constexpr int CPL = PARTS == 1 ? 2 : 1;              // rows in a lane's two columns
+template <typename T, int HD, int NT, bool NARROW>
+__global__ void __launch_bounds__(MOST_WARPS * 32, MmaShape<T, HD, NT, NARROW>::WARPS_SM / MOST_WARPS)
+attention_kv4_mma_kernel(const Kv4Attn p, int log_w, int tiles) {
+  using S = MmaShape<T, HD, NT, NARROW>;
+  constexpr int WPT = S::WPT, NWV = S::NWV, NB = S::NB, TK = S::TK, KS = S::KS, ROWS = S::ROWS, PARTS = S::PARTS, PER_ROW = S::PER_ROW, G16 = KS / 16;
+  constexpr int CPL = PER_ROW == 1 ? 2 : 1;            // rows in a lane's two columns
+  constexpr int NO = NARROW ? 2 : 4;                   // accumulator tiles of o^T per word of V
+  static_assert(!NARROW || NT == 1, "");
   extern __shared__ __align__(128) unsigned char sm[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, j = lane % 4;
-  const int W = 1 << log_w, wi = warp & (W - 1), split = blockIdx.x % p.splits;
+  const int MW = blockDim.x / 32, W = 1 << log_w, wi = warp & (W - 1), split = p.splits == 1 ? 0 : blockIdx.x % p.splits;
   unsigned char* ring = sm + warp * S::WARP_BYTES;
   uint64_t* bar = reinterpret_cast<uint64_t*>(sm + MW * S::WARP_BYTES) + warp * NSTG;
   if (lane < NSTG) tc05::mbar_init(&bar[lane], 1);
@@ -79,89 +89,106 @@ __global__ void __launch_bounds__(MW * 32) attention_kv4_mma_kernel(const Kv4Att
   __syncwarp();
   pdl_trigger();
   pdl_wait();
-  const long long unit = (long long)(blockIdx.x / p.splits) * (MW >> log_w) + (warp >> log_w);
-  const int tile = (int)(unit % tiles);
-  const long long pair = unit / tiles;
-  const int h = (int)(pair % p.d.heads), s = (int)(pair / p.d.heads);
-  int len = 0, cnt = 0;
-  if (s < p.d.slots) {
-    len = min(max(p.lens[s], 0), p.d.capacity);
-    cnt = p.counts ? min(max(p.counts[s], 0), p.n) : p.n;
-  }
-  const int r0 = tile * ROWS, rows = max(0, min(ROWS, cnt * p.group - r0));
-  // keys that row r sees; the last row sees most
-  auto sees = [&](int r) { return r < rows ? max(0, len - cnt + (r0 + r) / p.group + 1) : 0; };
-  const int most = rows > 0 ? sees(rows - 1) : 0, least = sees(0);
-  int see[NT][CPL];
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int c = 0; c < CPL; ++c) see[t][c] = sees(PARTS == 1 ? t * 8 + 2 * j + c : t * 4 + j);
+  const int unit = (p.splits == 1 ? blockIdx.x : blockIdx.x / p.splits) * (MW >> log_w) + (warp >> log_w);
+  const int tile = tiles == 1 ? 0 : unit % tiles, pair = tiles == 1 ? unit : unit / tiles;
+  const int s = pair / p.d.heads, h = pair - s * p.d.heads;
+  const bool here = s < p.d.slots;
 
-  // ---- the ring: lane x knows the slot of the warp's x-th tile (of 32 at a time), lane 0 issues
-  const int first = split * W + wi, step = p.splits * W, n_tiles = max(0, ceil_div(ceil_div(most, TK) - first, step));
-  const unsigned char* kc0 = p.d.kc + p.layer * p.d.code_layer + (long long)h * p.d.capacity * (HD / 2);
-  const unsigned char* vc0 = p.d.vc + p.layer * p.d.code_layer + (long long)h * p.d.capacity * (HD / 2);
-  const unsigned char* ks0 = p.d.ks + p.layer * p.d.scale_layer + (long long)h * p.d.capacity * NB;
-  const unsigned char* vs0 = p.d.vs + p.layer * p.d.scale_layer + (long long)h * p.d.capacity * NB;
+  // ---- the ring: lanes 0 .. 3 issue the copies of a tile, one each: key codes, key scales, value codes, value scales.  Lane x knows the
+  // slot of the warp's x-th tile (of 32 at a time).  The first tile is fetched before the length is known: it lies in the cache in any case.
+  const int first = split * W + wi, step = p.splits * W, cap_tiles = p.d.capacity / TK;
+  const unsigned char* src = lane == 0 ? p.d.kc : lane == 1 ? p.d.ks : lane == 2 ? p.d.vc : p.d.vs;
+  const int piece = lane & 1 ? S::SCALE_BYTES : S::CODE_BYTES;
+  const long long src_slot = lane & 1 ? p.d.scale_slot : p.d.code_slot;
+  const uint32_t dst = tc05::smem_u32(ring) + (lane & 1 ? S::CODE_BYTES : 0) + (lane & 2 ? S::CODE_BYTES + S::SCALE_BYTES : 0);
+  src += p.layer * (lane & 1 ? p.d.scale_layer : p.d.code_layer) + (long long)h * cap_tiles * piece;
   int slot_of = s, bad = 0;                            // bad: bit per stage, its page names no slot
   auto issue = [&](int i) {
-    if (i % 32 == 0) {
+    if (p.pages && i % 32 == 0) {
       const int t = first + (i + lane) * step;
-      slot_of = s;
-      if (p.pages && t * TK < most) slot_of = p.pages[(long long)s * (p.d.capacity / PAGE) + t * TK / PAGE];
+      slot_of = t < cap_tiles ? p.pages[(long long)s * (p.d.capacity / PAGE) + t * TK / PAGE] : s;
     }
     int slot = __shfl_sync(0xffffffffu, slot_of, i % 32);
     const int st = i % NSTG;
     bad &= ~(1 << st);
     if (slot < 0 || slot >= p.d.slots) { bad |= 1 << st; slot = s; }
-    if (lane == 0) {
-      unsigned char* dst = ring + st * S::STAGE;
-      const long long t = first + (long long)i * step, co = slot * p.d.code_slot + t * S::CODE_BYTES, so = slot * p.d.scale_slot + t * S::SCALE_BYTES;
-      tc05::mbar_expect_tx(&bar[st], S::STAGE);
-      tc05::bulk_load_1d(dst, kc0 + co, S::CODE_BYTES, &bar[st]);
-      tc05::bulk_load_1d(dst + S::CODE_BYTES, ks0 + so, S::SCALE_BYTES, &bar[st]);
-      tc05::bulk_load_1d(dst + S::CODE_BYTES + S::SCALE_BYTES, vc0 + co, S::CODE_BYTES, &bar[st]);
-      tc05::bulk_load_1d(dst + 2 * S::CODE_BYTES + S::SCALE_BYTES, vs0 + so, S::SCALE_BYTES, &bar[st]);
-    }
+    if (lane == 0) tc05::mbar_expect_tx(&bar[st], S::STAGE);
+    __syncwarp();
+    if (lane < 4)
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                   ::"r"(dst + st * S::STAGE), "l"(src + slot * src_slot + (long long)(first + i * step) * piece), "r"(piece), "r"(tc05::smem_u32(&bar[st])) : "memory");
   };
-  for (int i = 0; i < min(NSTG, n_tiles); ++i) issue(i);
+  const bool early = here && first < cap_tiles;
+  if (early) issue(0);
+  int len = 0, cnt = 0;
+  if (here) {
+    len = min(max(p.lens[s], 0), p.d.capacity);
+    cnt = p.counts ? min(max(p.counts[s], 0), p.n) : p.n;
+  }
+  const int r0 = tile * ROWS, rows = max(0, min(ROWS, cnt * p.group - r0));
+  // keys that row r sees; the last row sees most
+  auto token_of = [&](int r) { return p.n == 1 ? 0 : p.group == 1 ? r0 + r : (r0 + r) / p.group; };
+  auto sees = [&](int r) { return r < rows ? max(0, len - cnt + token_of(r) + 1) : 0; };
+  auto row_of = [&](int t, int c) { return PER_ROW == 1 ? t * 8 + 2 * j + c : PER_ROW == 2 ? t * 4 + j : j >> 1; };     // of this lane's columns
+  const int most = rows > 0 ? sees(rows - 1) : 0, least = sees(0);
+  int see[NT][CPL];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) see[t][c] = sees(row_of(t, c));
+  const int n_tiles = max(0, ceil_div(ceil_div(most, TK) - first, step));
+  for (int i = 1; i < min(NSTG, n_tiles); ++i) issue(i);
 
-  // ---- q: lane (g, j) holds the words j WPT .. of column g, as f16 of q 2^-e; c of a lane's own columns brings the scores to log2 units
+  // ---- q: lane (g, j) holds the words j WPT .. of column g, as f16 of q 2^-e; c of a lane's own columns brings the scores to log2 units.  c is
+  // positive (the scale's sign goes to q; without a scale all scores are 0), so the largest score is the largest product.
   uint32_t qf[NT][WPT][4];
   float cf[NT][CPL];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const int col = t * 8 + g, r = PARTS == 1 ? col : col / 2;
+    const int r = t * (8 / PER_ROW) + g / PER_ROW;
     float x[WPT][8], amax = 0.f;
-    const long long at = s * p.qb + (long long)((r0 + r) / p.group) * p.qt + (h * p.group + (r0 + r) % p.group) * p.qh;
+    const int token = token_of(r);
+    const T* q = reinterpret_cast<const T*>(p.q) + (s * p.qb + token * p.qt + (h * p.group + r0 + r - token * p.group) * p.qh + j * WPT * 8);
 #pragma unroll
     for (int i = 0; i < WPT; ++i) {
-      const int w = j * WPT + i;
 #pragma unroll
-      for (int y = 0; y < 8; ++y) {
-        x[i][y] = r < rows && w < S::WORDS ? to_f<T>(reinterpret_cast<const T*>(p.q)[at + w * 8 + y]) : 0.f;
-        amax = fmaxf(amax, fabsf(x[i][y]));
+      for (int y = 0; y < 8; ++y) x[i][y] = 0.f;
+      if (r < rows && j * WPT + i < S::WORDS) {
+        if (p.q_vec) {
+#pragma unroll
+          for (int y = 0; y < 8 / Pack<T>::N; ++y) {
+            Pack<T> v; v.load(q + i * 8 + y * Pack<T>::N);
+#pragma unroll
+            for (int z = 0; z < Pack<T>::N; ++z) x[i][y * Pack<T>::N + z] = v.v[z];
+          }
+        } else {
+#pragma unroll
+          for (int y = 0; y < 8; ++y) x[i][y] = to_f<T>(q[i * 8 + y]);
+        }
       }
+#pragma unroll
+      for (int y = 0; y < 8; ++y) amax = fmaxf(amax, fabsf(x[i][y]));
     }
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const int e = amax > 0.f && amax <= 3.402823466e38f ? ilogbf(amax) - 14 : 0;
+    // amax 2^-e lies in [2^14, 2^15); a row without a value of 2^-86 or more has no score of any size
+    const int e = max((int)(__float_as_uint(amax) >> 23) - 141, -100);
+    const float down = amax <= 3.402823466e38f ? (p.scale_log2 < 0.f ? -1.f : p.scale_log2 == 0.f ? 0.f : 1.f) * pow2(-e) : __int_as_float(0x7fc00000);
 #pragma unroll
     for (int i = 0; i < WPT; ++i)
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
-        const float a = ldexpf(x[i][2 * y], -e), b = ldexpf(x[i][2 * y + 1], -e);
+        const float a = x[i][2 * y] * down, b = x[i][2 * y + 1] * down;
         const uint32_t hi = f16x2(a, b);
         const float2 back = f16x2_f32(hi);
         qf[t][i][y] = PARTS == 1 || (g & 1) == 0 ? hi : f16x2(a - back.x, b - back.y);
       }
-    const float c = ldexpf(p.scale_log2, e + p.d.k_exp);
+    const float c = p.scale_log2 == 0.f ? 1.f : fmaxf(fabsf(p.scale_log2) * pow2(e / 2) * pow2(e - e / 2) * pow2(p.d.k_exp), 1e-37f);
 #pragma unroll
     for (int y = 0; y < CPL; ++y) cf[t][y] = __shfl_sync(0xffffffffu, c, 4 * (2 * j + y));
   }
 
-  float o[NWV][4][NT][4], m[NT][CPL], l[NT][CPL];
+  float o[NWV][NO][NT][4], m[NT][CPL], l[NT][CPL];     // m: of the products, not yet times c
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -169,11 +196,12 @@ __global__ void __launch_bounds__(MW * 32) attention_kv4_mma_kernel(const Kv4Att
 #pragma unroll
     for (int i = 0; i < NWV; ++i)
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < NO; ++u)
 #pragma unroll
         for (int y = 0; y < 4; ++y) o[i][u][t][y] = 0.f;
   }
   const int kperm = (g >> 1) + 4 * (g & 1);            // the key of row g of a tile: the keys of a lane's two columns of P^T then lie four apart in V
+  const uint32_t sel_a = g & 1 ? 0x1044 : 0x4410, sel_b = g & 1 ? 0x3244 : 0x4432;      // NARROW: (p, 0) or (0, p) of the lower and the upper half
   bool failed = false;
   for (int i = 0; i < n_tiles; ++i) {
     const int st = i % NSTG;
@@ -216,7 +244,7 @@ __global__ void __launch_bounds__(MW * 32) attention_kv4_mma_kernel(const Kv4Att
             int blk = (j * WPT + x) >> 1;
             if (S::WORDS % 4 != 0) blk = min(blk, NB - 1);
             const uint32_t two = e4m3x2_f16x2(ks[ka * NB + blk] | (uint32_t)ks[kb * NB + blk] << 8);
-            sa = __byte_perm(two, two, 0x1010); sb = __byte_perm(two, two, 0x3232);
+            sa = low2(two); sb = high2(two);
           }
           uint32_t ha[4], hb[4];
           unpack8(wa[x], ha); unpack8(wb[x], hb);
@@ -229,40 +257,50 @@ __global__ void __launch_bounds__(MW * 32) attention_kv4_mma_kernel(const Kv4Att
           }
         }
       }
-      // ---- softmax: sc[a][t][0], [1]: key kperm of group a, a lane's two columns; [2], [3]: key kperm + 8
-      uint32_t pf[G16][NT][2];
-      const bool masked = base + KS > least;
+      // ---- softmax: sc[a][t][0], [1]: key kperm of group a, a lane's two columns; [2], [3]: key kperm + 8.  Where the two columns belong to one
+      // row, [0] and [2] are brought to hold its scores.
+      if (PARTS == 2) {
+#pragma unroll
+        for (int a = 0; a < G16; ++a)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) { sc[a][t][0] += sc[a][t][1]; sc[a][t][2] += sc[a][t][3]; }
+      }
+      if (nan_tile) {
+#pragma unroll
+        for (int a = 0; a < G16; ++a)
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) sc[a][t][y] = __int_as_float(0x7fc00000);
+      }
+      if (base + KS > least) {
+#pragma unroll
+        for (int a = 0; a < G16; ++a)
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) {
+              if (base + a * 16 + kperm >= see[t][c]) sc[a][t][c] = -INFINITY;
+              if (base + a * 16 + kperm + 8 >= see[t][c]) sc[a][t][2 + c] = -INFINITY;
+            }
+      }
+      uint32_t pf[G16][NT][NARROW ? 4 : 2];            // NARROW: the two operands of the lower eight keys, then of the upper
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        float mx[CPL];
-#pragma unroll
-        for (int c = 0; c < CPL; ++c) mx[c] = -INFINITY;
-#pragma unroll
-        for (int a = 0; a < G16; ++a) {
-          float (&x)[4] = sc[a][t];
-          if (PARTS == 2) { x[0] += x[1]; x[2] += x[3]; }
-#pragma unroll
-          for (int c = 0; c < CPL; ++c) {
-            x[c] *= cf[t][c]; x[2 + c] *= cf[t][c];
-            if (nan_tile) x[c] = x[2 + c] = __int_as_float(0x7fc00000);
-            if (masked) {
-              if (base + a * 16 + kperm >= see[t][c]) x[c] = -INFINITY;
-              if (base + a * 16 + kperm + 8 >= see[t][c]) x[2 + c] = -INFINITY;
-            }
-            mx[c] = fmaxf(mx[c], fmaxf(x[c], x[2 + c]));
-          }
-        }
         bool moved = false;
-        float al[CPL], ref[CPL];
+        float mx[CPL], al[CPL], ref[CPL];
 #pragma unroll
         for (int c = 0; c < CPL; ++c) {
+          mx[c] = fmaxf(sc[0][t][c], sc[0][t][2 + c]);
+#pragma unroll
+          for (int a = 1; a < G16; ++a) mx[c] = fmaxf(mx[c], fmaxf(sc[a][t][c], sc[a][t][2 + c]));
           mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 4));
           mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 8));
           mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 16));
           const float mn = fmaxf(m[t][c], mx[c]), safe = mn == -INFINITY ? 0.f : mn;
-          al[c] = ex2(m[t][c] - safe);
+          al[c] = ex2((m[t][c] - safe) * cf[t][c]);
           moved |= mn != m[t][c];
-          ref[c] = safe - P_SHIFT;
+          ref[c] = P_SHIFT - safe * cf[t][c];
           m[t][c] = mn;
         }
         if (__any_sync(0xffffffffu, moved)) {
@@ -271,25 +309,37 @@ __global__ void __launch_bounds__(MW * 32) attention_kv4_mma_kernel(const Kv4Att
 #pragma unroll
           for (int x = 0; x < NWV; ++x)
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < NO; ++u)
 #pragma unroll
               for (int y = 0; y < 4; ++y) o[x][u][t][y] *= al[y % CPL];
         }
 #pragma unroll
         for (int a = 0; a < G16; ++a) {
-          float (&x)[4] = sc[a][t];
+          const float (&x)[4] = sc[a][t];
           uint32_t lo, hi;
-          if (PARTS == 1) {
-            const float p0 = ex2(x[0] - ref[0]), p1 = ex2(x[1] - ref[CPL - 1]), p2 = ex2(x[2] - ref[0]), p3 = ex2(x[3] - ref[CPL - 1]);
+          if (CPL == 2) {
+            const float2 c2 = make_float2(cf[t][0], cf[t][CPL - 1]), r2 = make_float2(ref[0], ref[CPL - 1]);
+            const float2 u = __ffma2_rn(make_float2(x[0], x[1]), c2, r2), v = __ffma2_rn(make_float2(x[2], x[3]), c2, r2);
+            const float p0 = ex2(u.x), p1 = ex2(u.y), p2 = ex2(v.x), p3 = ex2(v.y);
             l[t][0] += p0 + p2; l[t][CPL - 1] += p1 + p3;
             lo = f16x2(p0, p1); hi = f16x2(p2, p3);
           } else {
-            const float p0 = ex2(x[0] - ref[0]), p2 = ex2(x[2] - ref[0]);
+            const float p0 = ex2(fmaf(x[0], cf[t][0], ref[0])), p2 = ex2(fmaf(x[2], cf[t][0], ref[0]));
             l[t][0] += p0 + p2;
-            const float2 r = f16x2_f32(f16x2(p0, p2));
-            lo = f16x2(p0, p0 - r.x); hi = f16x2(p2, p2 - r.y);
+            if (PARTS == 1) { lo = f16x2(p0, p0); hi = f16x2(p2, p2); }
+            else {
+              const float2 r = f16x2_f32(f16x2(p0, p2));
+              const float q0 = p0 - r.x, q2 = p2 - r.y;
+              if (!NARROW) { lo = f16x2(p0, q0); hi = f16x2(p2, q2); }
+              else { lo = j & 1 ? f16x2(q0, q0) : f16x2(p0, p0); hi = j & 1 ? f16x2(q2, q2) : f16x2(p2, p2); }
+            }
           }
-          pf[a][t][0] = transpose8(lo); pf[a][t][1] = transpose8(hi);
+          lo = transpose8(lo); hi = transpose8(hi);
+          if (!NARROW) { pf[a][t][0] = lo; pf[a][t][1] = hi; }
+          else {
+            pf[a][t][0] = __byte_perm(lo, 0, sel_a); pf[a][t][1] = __byte_perm(lo, 0, sel_b);
+            pf[a][t][NARROW ? 2 : 0] = __byte_perm(hi, 0, sel_a); pf[a][t][NARROW ? 3 : 0] = __byte_perm(hi, 0, sel_b);
+          }
         }
       }
       // ---- o^T += V^T P^T
@@ -311,12 +361,25 @@ __global__ void __launch_bounds__(MW * 32) attention_kv4_mma_kernel(const Kv4Att
           // A NaN scale becomes 448 here: the key's scales are NaN as well and say so to the rows that see it, and to no other.  The same makes
           // whatever lies behind the last token a number, which its zero weight removes.
           const uint32_t s01 = min2(e4m3x2_f16x2(f[0] | (uint32_t)f[4 * NB] << 8), 0x5f005f00u), s23 = min2(e4m3x2_f16x2(f[8 * NB] | (uint32_t)f[12 * NB] << 8), 0x5f005f00u);
+          if (NARROW) {
+            const uint32_t sf[4] = {low2(s01), high2(s01), low2(s23), high2(s23)};
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const uint32_t a0 = mul2(__byte_perm(hv[0][u], hv[1][u], 0x5410), s01), a1 = mul2(__byte_perm(hv[0][u], hv[1][u], 0x7632), s01);
-            const uint32_t a2 = mul2(__byte_perm(hv[2][u], hv[3][u], 0x5410), s23), a3 = mul2(__byte_perm(hv[2][u], hv[3][u], 0x7632), s23);
+            for (int y = 0; y < 4; ++y)
 #pragma unroll
-            for (int t = 0; t < NT; ++t) mma_16816(o[x][u][t], a0, a1, a2, a3, pf[a][t][0], pf[a][t][1]);
+              for (int u = 0; u < 4; ++u) hv[y][u] = mul2(hv[y][u], sf[y]);
+#pragma unroll
+            for (int u = 0; u < NO; ++u) {
+              mma_16816(o[x][u][0], hv[0][2 * u & 3], hv[0][(2 * u + 1) & 3], hv[1][2 * u & 3], hv[1][(2 * u + 1) & 3], pf[a][0][0], pf[a][0][1]);
+              mma_16816(o[x][u][0], hv[2][2 * u & 3], hv[2][(2 * u + 1) & 3], hv[3][2 * u & 3], hv[3][(2 * u + 1) & 3], pf[a][0][NARROW ? 2 : 0], pf[a][0][NARROW ? 3 : 0]);
+            }
+          } else {
+#pragma unroll
+            for (int u = 0; u < NO; ++u) {
+              const uint32_t a0 = mul2(__byte_perm(hv[0][u], hv[1][u], 0x5410), s01), a1 = mul2(__byte_perm(hv[0][u], hv[1][u], 0x7632), s01);
+              const uint32_t a2 = mul2(__byte_perm(hv[2][u], hv[3][u], 0x5410), s23), a3 = mul2(__byte_perm(hv[2][u], hv[3][u], 0x7632), s23);
+#pragma unroll
+              for (int t = 0; t < NT; ++t) mma_16816(o[x][u][t], a0, a1, a2, a3, pf[a][t][0], pf[a][t][1]);
+            }
           }
         }
       }
@@ -328,7 +391,8 @@ __global__ void __launch_bounds__(MW * 32) attention_kv4_mma_kernel(const Kv4Att
     if (lane == 0) atomicExch(p.status, LLMB_ERR_TIMEOUT);
     for (int st = 0; st < NSTG; ++st) tc05::mbar_wait(&bar[st], 0);
   }
-  // ---- partial results: rows of HD sums, then maxima, then row sums, where the warp's ring was
+  if (early && n_tiles == 0 && !tc05::mbar_wait(&bar[0], 0) && lane == 0) atomicExch(p.status, LLMB_ERR_TIMEOUT);
+  // ---- partial results: rows of HD sums, then maxima (in log2 units), then row sums, where the warp's ring was
   float* po = reinterpret_cast<float*>(ring);
   float *pm = po + ROWS * HD, *pl = pm + ROWS;
   __syncwarp();
@@ -338,20 +402,29 @@ __global__ void __launch_bounds__(MW * 32) attention_kv4_mma_kernel(const Kv4Att
     for (int c = 0; c < CPL; ++c) {
       float v = l[t][c];
       v += __shfl_xor_sync(0xffffffffu, v, 4); v += __shfl_xor_sync(0xffffffffu, v, 8); v += __shfl_xor_sync(0xffffffffu, v, 16);
-      const int r = PARTS == 1 ? t * 8 + 2 * j + c : t * 4 + j;
-      if (g == 0) { pm[r] = m[t][c]; pl[r] = v; }
+      const int r = row_of(t, c);
+      const bool mine = PER_ROW < 4 || (j & 1) == 0;   // PER_ROW 4: two lanes hold a row's two parts
+      if (g == 0 && mine) { pm[r] = m[t][c] * cf[t][c]; pl[r] = v; }
 #pragma unroll
-      for (int x = 0; x < NWV; ++x)
+      for (int x = 0; x < NWV; ++x) {
+        const int w = g + 8 * x;
+        const bool in = r < rows && (S::WORDS % 8 == 0 || w < S::WORDS);
+        float* at = po + r * HD + w * 8;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int w = g + 8 * x;
-          if (r < rows && (S::WORDS % 8 == 0 || w < S::WORDS)) {
-            float2 v2;
-            if (PARTS == 1) v2 = make_float2(o[x][u][t][c], o[x][u][t][2 + c]);
-            else v2 = make_float2(o[x][u][t][0] + o[x][u][t][1], o[x][u][t][2] + o[x][u][t][3]);
-            *reinterpret_cast<float2*>(po + r * HD + w * 8 + 2 * u) = v2;
+        for (int u = 0; u < NO; ++u) {
+          const float (&y)[4] = o[x][u][t];
+          if (NARROW) {                                // a byte's two columns, then the next byte's
+            float4 v4 = make_float4(y[0], y[1], y[2], y[3]);
+            if (PARTS == 2) {
+              v4.x += __shfl_xor_sync(0xffffffffu, v4.x, 1); v4.y += __shfl_xor_sync(0xffffffffu, v4.y, 1);
+              v4.z += __shfl_xor_sync(0xffffffffu, v4.z, 1); v4.w += __shfl_xor_sync(0xffffffffu, v4.w, 1);
+            }
+            if (in && mine) *reinterpret_cast<float4*>(at + 4 * u) = v4;
+          } else if (in) {
+            *reinterpret_cast<float2*>(at + 2 * u) = PARTS == 1 ? make_float2(y[c], y[2 + c]) : make_float2(y[0] + y[1], y[2] + y[3]);
           }
         }
+      }
     }
   }
   if (W > 1) __syncthreads(); else __syncwarp();
@@ -359,42 +432,44 @@ __global__ void __launch_bounds__(MW * 32) attention_kv4_mma_kernel(const Kv4Att
   constexpr int PITCH = S::WARP_BYTES / 4;             // floats between two warps' parts
   float* u0 = reinterpret_cast<float*>(sm + (warp & ~(W - 1)) * S::WARP_BYTES);
   auto store = [&](int r, int c, float sum, float total) {
-    const long long at = s * p.ob + (long long)((r0 + r) / p.group) * p.ot + (h * p.group + (r0 + r) % p.group) * p.oh + c;
+    const int token = token_of(r);
+    const long long at = s * p.ob + token * p.ot + (h * p.group + r0 + r - token * p.group) * p.oh + c;
     reinterpret_cast<T*>(p.out)[at] = from_f<T>(total == 0.f ? 0.f : sum / total * vunit);
   };
-  if (p.splits == 1) {
-    for (int x = wi * 32 + lane; x < rows * HD; x += W * 32) {
-      const int r = x / HD, c = x % HD;
-      float mx = -INFINITY, sum = 0.f, total = 0.f;
-      for (int w = 0; w < W; ++w) mx = fmaxf(mx, u0[w * PITCH + ROWS * HD + r]);
-      const float ref = mx == -INFINITY ? 0.f : mx;
-      for (int w = 0; w < W; ++w) {
-        const float f = ex2(u0[w * PITCH + ROWS * HD + r] - ref);
-        sum += u0[w * PITCH + x] * f; total += u0[w * PITCH + ROWS * HD + ROWS + r] * f;
-      }
-      store(r, c, sum, total);
-    }
-    return;
-  }
-  // a cluster per unit (W = MW): each block leaves its parts as they are, and finishes a share of the elements from everybody's
-  cg::cluster_group cluster = cg::this_cluster();
-  cluster.sync();
-  for (int x = split * (MW * 32) + threadIdx.x; x < rows * HD; x += p.splits * MW * 32) {
+  __shared__ float um[ROWS], ul[ROWS], share[MOST_SPLITS][ROWS];
+  for (int x = wi * 32 + lane; x < rows * HD; x += W * 32) {
     const int r = x / HD, c = x % HD;
     float mx = -INFINITY, sum = 0.f, total = 0.f;
-    for (int k = 0; k < p.splits; ++k) {
-      const float* u = cluster.map_shared_rank(u0, k);
-      for (int w = 0; w < MW; ++w) mx = fmaxf(mx, u[w * PITCH + ROWS * HD + r]);
-    }
+    for (int w = 0; w < W; ++w) mx = fmaxf(mx, u0[w * PITCH + ROWS * HD + r]);
     const float ref = mx == -INFINITY ? 0.f : mx;
-    for (int k = 0; k < p.splits; ++k) {
-      const float* u = cluster.map_shared_rank(u0, k);
-      for (int w = 0; w < MW; ++w) {
-        const float f = ex2(u[w * PITCH + ROWS * HD + r] - ref);
-        sum += u[w * PITCH + x] * f; total += u[w * PITCH + ROWS * HD + ROWS + r] * f;
-      }
+    for (int w = 0; w < W; ++w) {
+      const float f = ex2(u0[w * PITCH + ROWS * HD + r] - ref);
+      sum += u0[w * PITCH + x] * f; total += u0[w * PITCH + ROWS * HD + ROWS + r] * f;
     }
-    store(r, c, sum, total);
+    if (p.splits == 1) store(r, c, sum, total);
+    else {                                             // a unit per cluster: W is the whole block
+      u0[x] = sum;
+      if (c == 0) { um[r] = mx; ul[r] = total; }
+    }
+  }
+  if (p.splits == 1) return;
+  // The blocks of a cluster: each has its part of every row; each finishes a share of the elements from everybody's.
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  for (int x = threadIdx.x; x < rows * p.splits; x += blockDim.x) {
+    const int r = x / p.splits, k = x % p.splits;
+    float mx = -INFINITY, total = 0.f;
+    for (int y = 0; y < p.splits; ++y) mx = fmaxf(mx, *cluster.map_shared_rank(&um[r], y));
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    for (int y = 0; y < p.splits; ++y) total += *cluster.map_shared_rank(&ul[r], y) * ex2(*cluster.map_shared_rank(&um[r], y) - ref);
+    share[k][r] = total == 0.f ? 0.f : ex2(*cluster.map_shared_rank(&um[r], k) - ref) / total;
+  }
+  __syncthreads();
+  for (int x = split * blockDim.x + threadIdx.x; x < rows * HD; x += p.splits * blockDim.x) {
+    const int r = x / HD;
+    float sum = 0.f;
+    for (int k = 0; k < p.splits; ++k) sum += cluster.map_shared_rank(u0, k)[x] * share[k][r];
+    store(r, x % HD, sum, 1.f);
   }
   cluster.sync();                                      // no block leaves while another reads its shared memory
 }
@@ -404,35 +479,42 @@ inline int allow_smem(unsigned long long& done, const void* kernel, int bytes) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && !(dev < 64 && (done >> dev & 1))) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);      // clusters of 16
     if (e == cudaSuccess && dev < 64) done |= 1ull << dev;
   }
   return (int)e;
 }
 
-template <typename T, int HD, int NT>
+template <typename T, int HD, int NT, bool NARROW>
 int run_mma(Kv4Attn p, cudaStream_t st) {
-  using S = MmaShape<T, HD, NT>;
-  static unsigned long long attr = 0;                  // devices on which the kernel may take its shared memory
-  if (const int e = allow_smem(attr, (const void*)attention_kv4_mma_kernel<T, HD, NT>, S::SMEM)) return e;
+  using S = MmaShape<T, HD, NT, NARROW>;
+  const auto kernel = attention_kv4_mma_kernel<T, HD, NT, NARROW>;
+  static unsigned long long attr = 0;                  // devices on which the kernel has its attributes
+  if (const int e = allow_smem(attr, (const void*)kernel, MOST_WARPS * S::SMEM_WARP)) return e;
   const long long tiles = ceil_div_ll((long long)p.n * p.group, S::ROWS), units = tiles * p.d.heads * p.d.slots;
-  // One warp a unit where there are enough of them to fill the chip (three blocks of four warps on an SM), else two, four, and a cluster.
-  const long long want = (long long)sm_count() * 12;
-  const int most = ceil_div(p.d.capacity, S::TK);      // no more warps than tiles
-  int log_w = 0;
-  while (log_w < 2 && (units << log_w) < want && (1 << log_w) < most) ++log_w;
+  if (units * MOST_WARPS * 16 > 0x7fffffffLL) return LLMB_ERR_BAD_ARG;
+  // How many warps share a unit.  Units that fill the chip get one warp each, or two where a second round would be a short one (256 x 16
+  // heads of 64, up to 1024 tokens: 63 us with one, 56 with two, 57 with four, 67 with eight; 1024 x 16, up to 512: 106, 112, 130, 184); fewer
+  // get up to eight, as long as all warps fit on the chip at once (32 x 12, up to 777 tokens: 16, 12.7, 11.2, 8.9; 64 x 12: 26, 23, 17, 18), and
+  // then a cluster of blocks, which costs 1 - 3 us and pays where each warp keeps three tiles (4 x 8 heads of 128, 32001 tokens: 153 us in one
+  // block, 82, 62, 37 in 2, 4, 8; 1 x 12, 1000 tokens: 5.3 in one block, 6.2 in two).
+  const long long fit = (long long)sm_count() * S::WARPS_SM;
+  const int most = ceil_div(p.d.capacity, S::TK);
+  int log_w = units > fit && units <= 2 * fit && most > 1 ? 1 : 0;
+  while (log_w < 3 && (units << (log_w + 1)) <= fit && (2 << log_w) <= most) ++log_w;
   p.splits = 1;
-  if (log_w == 2) while (p.splits < 8 && units * 4 * p.splits < want && p.splits * 4 < most) p.splits *= 2;
-  const long long blocks = ceil_div_ll(units << log_w, MW) * p.splits;
-  if (blocks > 0x7fffffffLL || tiles > 0x7fffffffLL) return LLMB_ERR_BAD_ARG;
-  return launch_pdl_cluster(dim3(p.splits), attention_kv4_mma_kernel<T, HD, NT>, dim3((unsigned)blocks), MW * 32, S::SMEM, st, p, log_w, (int)tiles);
+  if (log_w == 3) while (p.splits < MOST_SPLITS && units * 16 * p.splits <= fit && p.splits * 48 <= most) p.splits *= 2;
+  const int warps = log_w == 3 ? 8 : 4;
+  return launch_pdl_cluster(dim3(p.splits), kernel, dim3((unsigned)(ceil_div_ll(units << log_w, warps) * p.splits)), warps * 32, warps * S::SMEM_WARP, st, p, log_w, (int)tiles);
 }
 template <typename T, int HD>
 int run(const Kv4Attn& p, cudaStream_t st) {
   const long long rows = (long long)p.n * p.group;
   constexpr int R8 = sizeof(T) == 4 ? 4 : 8, MOST = HD <= 64 ? 4 : 2;
-  if (rows <= R8) return run_mma<T, HD, 1>(p, st);
-  if (rows <= 2 * R8 || MOST == 2) return run_mma<T, HD, 2>(p, st);
-  return run_mma<T, HD, MOST>(p, st);
+  if (rows <= R8 / 2) return run_mma<T, HD, 1, true>(p, st);
+  if (rows <= R8) return run_mma<T, HD, 1, false>(p, st);
+  if (rows <= 2 * R8 || MOST == 2) return run_mma<T, HD, 2, false>(p, st);
+  return run_mma<T, HD, MOST, false>(p, st);
 }
 template <typename T>
 int run_type(const Kv4Attn& p, cudaStream_t st) {
@@ -459,6 +541,8 @@ struct Kv4AttendArgs {
 LLMB_API int llmb_attention_kv4(const Kv4Desc* d, const Kv4AttendArgs* a, cudaStream_t st) {
   if (a->heads % d->heads) return LLMB_ERR_BAD_ARG;
   Kv4Attn p{*d, a->out, a->q, a->lens, a->counts, a->pages, a->layer, a->n, a->heads / d->heads, 1, a->scale * 1.4426950408889634f,
-            a->qb, a->qt, a->qh, a->ob, a->ot, a->oh, a->status};
+            a->qb, a->qt, a->qh, a->ob, a->ot, a->oh, a->status, false};
+  const int elt = a->dtype == LLMB_BF16 ? 2 : 4;
+  p.q_vec = ((reinterpret_cast<uintptr_t>(a->q) | (uintptr_t)(a->qb * elt) | (uintptr_t)(a->qt * elt) | (uintptr_t)(a->qh * elt)) & 15) == 0;
   return a->dtype == LLMB_BF16 ? run_type<__nv_bfloat16>(p, st) : run_type<float>(p, st);
 }

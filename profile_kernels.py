@@ -8,6 +8,8 @@
     python profile_kernels.py nvfp4       # NVFP4 operands (maxima, both orientations) and block-scaled GEMMs, 8192 x 1600 x 6400
     python profile_kernels.py fp8b        # block-scaled FP8 operands (both orientations) and GEMMs, 8192 x 1280 x 5120
     python profile_kernels.py lmhead      # LM-head GEMM on 8192 rows + fused softmax/cross-entropy
+    python profile_kernels.py kv4         # attention over the 4-bit cache: 256 x 16 heads of 1000 tokens, shared heads of 32000, a prompt; append, read back, reorder
+    python profile_kernels.py beam        # beam selection, 48 items of 8 beams over 50257 fp32 logits
     python profile_kernels.py layernorm   # LayerNorm forward + backward on 65536 x 768
     python profile_kernels.py fusedpull   # a layer GEMM that pulls its own weight (four emulated owners) with its copier warps
     python profile_kernels.py fusedgather # the all-gather-fused GEMM with four "ranks" emulated on ONE GPU: the peers'
@@ -92,6 +94,42 @@ def case_lmhead(reps):
     for _ in range(reps):
         ops.matmul_fwd(logits, x, w)
         ops.fused_classifier(logits, losses, tgt, 1.0 / rows, V)
+
+
+def case_kv4(reps):
+    def cache(layers, S, H, T, hd):
+        c = ops.KV4Cache.empty(layers, S, H, T, hd)
+        for t in (c.k_codes, c.v_codes):
+            t.random_(0, 256)
+        for t in (c.k_scales, c.v_scales):
+            t.random_(40, 64)
+        return c
+
+    def attend(c, heads, n, length):
+        q = torch.randn(c.slots, n, heads, c.head_size, device="cuda").bfloat16()
+        ops.attention_kv4(torch.empty_like(q), q, c, 0, torch.full((c.slots,), length, dtype=torch.int32, device="cuda"))
+
+    wide, shared, prompt, beams = cache(1, 256, 16, 1000, 64), cache(1, 4, 8, 32000, 128), cache(1, 16, 12, 1000, 64), cache(24, 64, 16, 800, 64)
+    qkv = torch.randn(16, 1000, 3, 12, 64, device="cuda").bfloat16()
+    ko, vo = (torch.empty(24, 64, 64, 16, 64, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    pages, lens = beams.own_pages(), torch.full((64,), 800, dtype=torch.int32, device="cuda")
+    parents = torch.randint(0, 8, (8, 8), dtype=torch.int32, device="cuda")
+    zeros = torch.zeros(64, dtype=torch.int32, device="cuda")
+    for _ in range(reps):
+        attend(wide, 16, 1, 1000)
+        attend(shared, 32, 1, 32000)
+        attend(prompt, 12, 1000, 1000)
+        ops.kv4_append(prompt, 0, qkv[:, :, 1], qkv[:, :, 2], zeros[:16])
+        ops.kv4_reorder(beams, pages, lens, parents)
+        ops.kv4_values(ko, vo, beams, None, zeros)
+
+
+def case_beam(reps):
+    B, K, V = 48, 8, 50257
+    logits, scores = torch.randn(B * K, V, device="cuda"), torch.zeros(B, K, device="cuda")
+    tokens, parents = (torch.empty(B, K, dtype=torch.int32, device="cuda") for _ in range(2))
+    for _ in range(reps):
+        ops.beam_select(torch.empty_like(scores), tokens, parents, logits, scores, V)
 
 
 def case_layernorm(reps):
@@ -204,7 +242,7 @@ def case_fp8b(reps):
         lowp.matmul_bwd_fp8_block(dinp, dw, None, d, x, w)
 
 
-CASES = {"fp8b": case_fp8b, "small": case_small, "f32attn": case_f32attn, "nvfp4": case_nvfp4, "fusedgather": case_fusedgather, "fusedpull": case_fusedpull, "attn": case_attn, "gemm": case_gemm, "lmhead": case_lmhead, "layernorm": case_layernorm}
+CASES = {"kv4": case_kv4, "beam": case_beam, "fp8b": case_fp8b, "small": case_small, "f32attn": case_f32attn, "nvfp4": case_nvfp4, "fusedgather": case_fusedgather, "fusedpull": case_fusedpull, "attn": case_attn, "gemm": case_gemm, "lmhead": case_lmhead, "layernorm": case_layernorm}
 
 if __name__ == "__main__":
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
