@@ -40,26 +40,38 @@ template <typename T, bool VEC> __device__ __forceinline__ void store16(T* p, co
   }
 }
 
+// x / s correctly rounded from r = 1 / s correctly rounded: one step on the remainder (Markstein).  |x / s| stays far from both ends of fp32.
+__device__ __forceinline__ float divide(float x, float s, float r) {
+  const float q = x * r;
+  return fmaf(fmaf(-q, s, x), r, q);
+}
+
 // One thread per block of 16 values; the threads of a row's key blocks and of its value blocks are neighbours (GROUP of them, some idle where
 // 2 HD / 16 is no power of two) because a non-finite value in one block marks all of them.  Rows are counted (slot, head, token), the token
-// fastest, so that a warp's stores are dense in the cache.  The quotients are true divisions: x / scale is then a tie between two levels exactly
-// where it is one in the reals (a midpoint has 3 bits, a scale 4, so x would have to be their product), and the conversion rounds it to even.
+// fastest, so that a warp's stores are dense in the cache.
+// The codes are those of the exact quotients x / s, s the scale.  A tie between two levels is a product of a midpoint's 3 bits and the scale's 4.
+// The correctly rounded quotient is a midpoint only where x / s is one; a product with the rounded reciprocal is not (fl(1 / 0.875) 0.75 x 0.875
+// lies above 0.75), and a true division costs eight operations against three.
 template <typename T, int HD, bool VEC>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Desc d, int layer, const T* __restrict__ k, const T* __restrict__ v,
                                                          const int* __restrict__ start, const int* __restrict__ counts, int n, RowStrides sk, RowStrides sv) {
   pdl_trigger();
   pdl_wait();
-  constexpr int NB = HD / BLOCK, GROUP = NB <= 2 ? 4 : NB <= 4 ? 8 : 16;
-  const long long rows = (long long)d.slots * d.heads * n;
+  constexpr int NB = HD / BLOCK, GROUP = NB <= 2 ? 4 : NB <= 4 ? 8 : 16, ROWS = 256 / GROUP;
+  const unsigned rows = (unsigned)d.slots * d.heads * n;        // below 2^31 (host)
   const int at = threadIdx.x % GROUP;
   const bool is_v = at >= NB;
   const int blk = is_v ? at - NB : at;
+  const RowStrides st = is_v ? sv : sk;
+  const T* const from = (is_v ? v : k) + blk * BLOCK;
+  const int e = is_v ? d.v_exp : d.k_exp;
+  const float unit = pow2(e), per_unit = pow2(-e);
+  uint8_t* const codes = (is_v ? d.vc : d.kc) + layer * d.code_layer + blk * 8;
+  uint8_t* const scales = (is_v ? d.vs : d.ks) + layer * d.scale_layer + blk;
   // whole groups walk the rows together, so the shuffles below have all their lanes
-  for (long long r0 = (long long)blockIdx.x * (256 / GROUP); r0 < rows; r0 += (long long)gridDim.x * (256 / GROUP)) {
-    const long long r = r0 + threadIdx.x / GROUP;
-    const int i = (int)(r % n);
-    const long long sh = r / n;
-    const int h = (int)(sh % d.heads), s = (int)(sh / d.heads);
+  for (unsigned r0 = blockIdx.x * ROWS; r0 < rows; r0 += gridDim.x * ROWS) {
+    const unsigned r = r0 + threadIdx.x / GROUP, sh = r / (unsigned)n, s = sh / (unsigned)d.heads;
+    const int i = (int)(r - sh * n), h = (int)(sh - s * d.heads);
     bool live = r < rows && at < 2 * NB;
     long long pos = 0;
     if (live) {
@@ -70,77 +82,85 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Desc d, int la
     float amax = 0.f;
     bool bad = false;
     if (live) {
-      const RowStrides& st = is_v ? sv : sk;
-      load16<T, VEC>(x, (is_v ? v : k) + s * st.b + i * st.t + h * st.h + blk * BLOCK);
+      load16<T, VEC>(x, from + s * st.b + i * st.t + h * st.h);
 #pragma unroll
       for (int j = 0; j < 16; ++j) { bad |= !(fabsf(x[j]) <= 3.402823466e38f); amax = fmaxf(amax, fabsf(x[j])); }
     }
 #pragma unroll
     for (int o = 1; o < GROUP; o <<= 1) bad |= __shfl_xor_sync(0xffffffffu, (int)bad, o) != 0;
     if (!live) continue;
-    const int e = is_v ? d.v_exp : d.k_exp;
-    const uint32_t sc = e4m3(__fdiv_rn(amax * pow2(-e), 6.0f));
-    const float s32 = e4m3_f32(sc) * pow2(e);
+    const uint32_t sc = e4m3(__fdiv_rn(amax * per_unit, 6.0f));
+    const float s32 = e4m3_f32(sc) * unit, inv = __frcp_rn(s32);
     uint32_t lo = 0, hi = 0;
     if (!bad && sc != 0) {
+      if (sc == 0x7e) {                                // the largest scale: what saturates stays in range
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = fminf(fmaxf(x[j], -8.f * s32), 8.f * s32);
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = divide(x[j], s32, inv);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        lo |= e2m1x2(__fdiv_rn(x[2 * j], s32), __fdiv_rn(x[2 * j + 1], s32)) << (8 * j);
-        hi |= e2m1x2(__fdiv_rn(x[8 + 2 * j], s32), __fdiv_rn(x[9 + 2 * j], s32)) << (8 * j);
+        lo |= e2m1x2(x[2 * j], x[2 * j + 1]) << (8 * j);
+        hi |= e2m1x2(x[8 + 2 * j], x[9 + 2 * j]) << (8 * j);
       }
     }
     const long long row = (long long)h * d.capacity + pos;
-    uint8_t* codes = (is_v ? d.vc : d.kc) + layer * d.code_layer + s * d.code_slot + row * (HD / 2) + blk * 8;
-    uint8_t* scales = (is_v ? d.vs : d.ks) + layer * d.scale_layer + s * d.scale_slot + row * NB + blk;
-    *reinterpret_cast<uint2*>(codes) = make_uint2(lo, hi);
-    *scales = bad ? 0x7f : (uint8_t)sc;
+    *reinterpret_cast<uint2*>(codes + s * d.code_slot + row * (HD / 2)) = make_uint2(lo, hi);
+    scales[s * d.scale_slot + row * NB] = bad ? 0x7f : (uint8_t)sc;
   }
 }
 
-// One thread per block of 16 values of both the key and the value; the blocks of a row, then its heads, then its tokens are neighbours, so
-// that the stores, which are most of the bytes, are dense where the outputs are.
+// One thread per 16 bytes of an output, of both the key and the value; the pieces of a row, then its heads, then its tokens are neighbours: the
+// stores, which are most of the bytes, are dense where the outputs are.  A block stays with one slot of one layer.
 template <typename T, int HD, bool VEC>
 __global__ void __launch_bounds__(256) kv4_values_kernel(const Kv4Desc d, int layer, T* __restrict__ ko, T* __restrict__ vo, const int* __restrict__ start,
                                                          const int* __restrict__ pages, int n, long long out_layer, RowStrides sk, RowStrides sv) {
   pdl_trigger();
   pdl_wait();
-  constexpr int NB = HD / BLOCK;
-  const int layers = layer < 0 ? d.layers : 1;
-  const long long total = (long long)layers * d.slots * n * d.heads * NB;
-  for (long long x = (long long)blockIdx.x * 256 + threadIdx.x; x < total; x += (long long)gridDim.x * 256) {
-    const int blk = (int)(x % NB);
-    long long r = x / NB;
-    const int h = (int)(r % d.heads); r /= d.heads;
-    const int i = (int)(r % n); r /= n;
-    const int s = (int)(r % d.slots), l = (int)(r / d.slots);
-    const long long pos = (long long)start[s] + i;
-    float kx[16], vx[16];
-    if (pos < 0 || pos >= d.capacity) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) kx[j] = vx[j] = 0.f;
-    } else {
-      int slot = s;
-      if (pages) slot = pages[(long long)s * (d.capacity / PAGE) + pos / PAGE];
-      if (slot < 0 || slot >= d.slots) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) kx[j] = vx[j] = __int_as_float(0x7fc00000);
-      } else {
-        const long long row = (long long)h * d.capacity + pos;
-        const long long c = (layer < 0 ? l : layer) * d.code_layer + slot * d.code_slot + row * (HD / 2) + blk * 8;
-        const long long f = (layer < 0 ? l : layer) * d.scale_layer + slot * d.scale_slot + row * NB + blk;
-        const uint2 kc = *reinterpret_cast<const uint2*>(d.kc + c), vc = *reinterpret_cast<const uint2*>(d.vc + c);
-        const float ks = e4m3_f32(d.ks[f]) * pow2(d.k_exp), vs = e4m3_f32(d.vs[f]) * pow2(d.v_exp);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float2 a = f16x2_f32(e2m1x2_f16x2(((j < 4 ? kc.x : kc.y) >> (8 * (j & 3))) & 0xff));
-          const float2 b = f16x2_f32(e2m1x2_f16x2(((j < 4 ? vc.x : vc.y) >> (8 * (j & 3))) & 0xff));
-          kx[2 * j] = a.x * ks; kx[2 * j + 1] = a.y * ks;
-          vx[2 * j] = b.x * vs; vx[2 * j + 1] = b.y * vs;
+  constexpr int NB = HD / BLOCK, N = 16 / sizeof(T), PIECES = HD / N;
+  const unsigned total = (unsigned)n * d.heads * PIECES, planes = (layer < 0 ? d.layers : 1) * d.slots;      // below 2^31 (host)
+  for (unsigned plane = blockIdx.y; plane < planes; plane += gridDim.y) {
+    const int l = plane / d.slots, s = plane - l * d.slots;
+    const long long first = start[s];
+    const long long cl = (layer < 0 ? l : layer) * d.code_layer, fl = (layer < 0 ? l : layer) * d.scale_layer;
+    for (unsigned x = blockIdx.x * 256 + threadIdx.x; x < total; x += gridDim.x * 256) {
+      const unsigned row_of = x / PIECES, i = row_of / d.heads;
+      const int piece = x - row_of * PIECES, h = row_of - i * d.heads;
+      const long long pos = first + i;
+      float kx[N], vx[N];
+      float ks = 0.f, vs = 0.f;
+      uint32_t kw = 0, vw = 0;
+      if (pos >= 0 && pos < d.capacity) {
+        int slot = s;
+        if (pages) slot = pages[(long long)s * (d.capacity / PAGE) + pos / PAGE];
+        if (slot < 0 || slot >= d.slots) ks = vs = __int_as_float(0x7fc00000);
+        else {
+          const long long row = (long long)h * d.capacity + pos;
+          const long long c = cl + slot * d.code_slot + row * (HD / 2) + piece * (N / 2), f = fl + slot * d.scale_slot + row * NB + piece * N / BLOCK;
+          if (N == 8) { kw = *reinterpret_cast<const uint32_t*>(d.kc + c); vw = *reinterpret_cast<const uint32_t*>(d.vc + c); }
+          else { kw = *reinterpret_cast<const uint16_t*>(d.kc + c); vw = *reinterpret_cast<const uint16_t*>(d.vc + c); }
+          ks = e4m3_f32(d.ks[f]) * pow2(d.k_exp); vs = e4m3_f32(d.vs[f]) * pow2(d.v_exp);
         }
       }
+#pragma unroll
+      for (int j = 0; j < N / 2; ++j) {
+        const float2 a = f16x2_f32(e2m1x2_f16x2((kw >> (8 * j)) & 0xff)), b = f16x2_f32(e2m1x2_f16x2((vw >> (8 * j)) & 0xff));
+        kx[2 * j] = a.x * ks; kx[2 * j + 1] = a.y * ks;
+        vx[2 * j] = b.x * vs; vx[2 * j + 1] = b.y * vs;
+      }
+      T* const kp = ko + l * out_layer + s * sk.b + i * sk.t + h * sk.h + piece * N;
+      T* const vp = vo + l * out_layer + s * sv.b + i * sv.t + h * sv.h + piece * N;
+      if (VEC) {
+        Pack<T> a, b;
+#pragma unroll
+        for (int j = 0; j < N; ++j) { a.v[j] = kx[j]; b.v[j] = vx[j]; }
+        a.store(kp); b.store(vp);
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) { kp[j] = from_f<T>(kx[j]); vp[j] = from_f<T>(vx[j]); }
+      }
     }
-    store16<T, VEC>(ko + l * out_layer + s * sk.b + i * sk.t + h * sk.h + blk * BLOCK, kx);
-    store16<T, VEC>(vo + l * out_layer + s * sv.b + i * sv.t + h * sv.h + blk * BLOCK, vx);
   }
 }
 
@@ -151,59 +171,42 @@ __device__ __forceinline__ int parent_of(const int* parents, int item, int j, in
 }
 __device__ __forceinline__ int length_of(const int* lens, int slot, int capacity) { return min(max(lens[slot], 0), capacity); }
 
-// The page that is being filled: one block per (item, head, layer) takes 16-byte pieces of every beam's page into shared memory, then every beam
-// that has another parent writes its parent's.  Beams of an item are read before any of them is written; items, heads and layers do not meet.
-constexpr int REORDER_THREADS = 256;
-__global__ void __launch_bounds__(REORDER_THREADS) kv4_reorder_kernel(const Kv4Desc d, const int* __restrict__ lens, const int* __restrict__ parents, int K) {
+// The page that is being filled: its used part is contiguous in each of the four tensors.  One block per (item, head, layer); a thread takes the
+// same 16 bytes of every beam's page that is somebody's parent into a column of shared memory of its own, then gives every beam with another
+// parent its parent's.  So no thread waits for another, and everything is read before it is written: other threads write other bytes.
+constexpr int REORDER_PIECES = 2048;                  // 16-byte pieces in shared memory: one of each beam for every thread
+__global__ void __launch_bounds__(256) kv4_reorder_kernel(const Kv4Desc d, const int* __restrict__ lens, const int* __restrict__ parents, int K) {
   pdl_trigger();
   pdl_wait();
-  constexpr int PIECES = 512;                          // 16-byte pieces in shared memory at a time
-  __shared__ uint4 buf[PIECES];
-  const int item = blockIdx.x, h = blockIdx.y, layer = blockIdx.z;
-  const int cb = d.head_size / 2, sb = d.head_size / BLOCK;
-  // pieces of one beam's page: codes and scales of keys, then of values (all multiples of 16 bytes for 64 tokens)
-  const int code_pieces = PAGE * cb / 16, scale_pieces = PAGE * sb / 16, all = 2 * (code_pieces + scale_pieces);
-  const int per = PIECES / K;                          // pieces of each beam at a time (K <= 64)
-  auto address = [&](int slot, int page, int x, int* token) -> uint8_t* {
-    const bool is_v = x >= code_pieces + scale_pieces;
-    if (is_v) x -= code_pieces + scale_pieces;
-    const bool is_scale = x >= code_pieces;
-    if (is_scale) x -= code_pieces;
-    const int bytes = is_scale ? sb : cb;
-    *token = x * 16 / bytes;                           // the first token that has a byte in the piece
-    uint8_t* base = is_scale ? (is_v ? d.vs : d.ks) + layer * d.scale_layer + slot * d.scale_slot : (is_v ? d.vc : d.kc) + layer * d.code_layer + slot * d.code_slot;
-    return base + ((long long)h * d.capacity + (long long)page * PAGE) * bytes + x * 16;
-  };
-  for (int x0 = 0; x0 < all; x0 += per) {
-    const int w = min(per, all - x0);
-    for (int t = threadIdx.x; t < w * K; t += REORDER_THREADS) {
-      const int j = t / w, x = x0 + t % w, slot = item * K + j;
-      const int len = length_of(lens, slot, d.capacity);
-      int token;
-      if (len % PAGE == 0) continue;
-      uint8_t* a = address(slot, len / PAGE, x, &token);
-      if (token < len % PAGE) buf[j * per + t % w] = *reinterpret_cast<const uint4*>(a);
-    }
-    __syncthreads();
-    for (int t = threadIdx.x; t < w * K; t += REORDER_THREADS) {
-      const int j = t / w, x = x0 + t % w, of = parent_of(parents, item, j, K);
-      const int len = length_of(lens, item * K + of, d.capacity), rest = len % PAGE;
-      if (of == j || rest == 0) continue;
-      int token;
-      uint8_t* a = address(item * K + j, len / PAGE, x, &token);
-      if (token >= rest) continue;
-      // a piece of scales may hold tokens behind the last one: those stay as they are
-      const bool is_scale = x % (code_pieces + scale_pieces) >= code_pieces;
-      const int bytes = is_scale ? sb : cb;
-      const int first = (x % (code_pieces + scale_pieces) - (is_scale ? code_pieces : 0)) * 16, keep = rest * bytes - first;
-      const uint4 val = buf[of * per + t % w];
+  __shared__ uint4 buf[REORDER_PIECES];
+  __shared__ int of[64], len[64], wanted[64];
+  const int item = blockIdx.x, h = blockIdx.y, layer = blockIdx.z, j0 = threadIdx.x;
+  for (int j = j0; j < K; j += blockDim.x) { of[j] = parent_of(parents, item, j, K); len[j] = length_of(lens, item * K + j, d.capacity); wanted[j] = 0; }
+  __syncthreads();
+  for (int j = j0; j < K; j += blockDim.x) if (of[j] != j && len[of[j]] % PAGE) wanted[of[j]] = 1;
+  __syncthreads();
+  const int cb = d.head_size / 2, sb = d.head_size / BLOCK, code_pieces = PAGE * cb / 16, scale_pieces = PAGE * sb / 16;
+  for (int x = threadIdx.x; x < 2 * (code_pieces + scale_pieces); x += blockDim.x) {
+    const int y = x < code_pieces + scale_pieces ? x : x - code_pieces - scale_pieces;
+    const bool is_v = y != x, is_scale = y >= code_pieces;
+    const int bytes = is_scale ? sb : cb, first = (is_scale ? y - code_pieces : y) * 16;           // bytes of a token; the piece's first byte
+    const long long slot_stride = is_scale ? d.scale_slot : d.code_slot;
+    uint8_t* const base = (is_scale ? (is_v ? d.vs : d.ks) + layer * d.scale_layer : (is_v ? d.vc : d.kc) + layer * d.code_layer) +
+                          item * K * slot_stride + (long long)h * d.capacity * bytes + first;
+    auto place = [&](int j, int n) { return base + j * slot_stride + (long long)(n / PAGE) * PAGE * bytes; };
+    for (int j = 0; j < K; ++j)
+      if (wanted[j] && first < (len[j] % PAGE) * bytes) buf[j * blockDim.x + threadIdx.x] = *reinterpret_cast<const uint4*>(place(j, len[j]));
+    for (int j = 0; j < K; ++j) {
+      const int p = of[j], n = len[p], keep = (n % PAGE) * bytes - first;
+      if (p == j || keep <= 0) continue;
+      const uint4 val = buf[p * blockDim.x + threadIdx.x];
+      uint8_t* const a = place(j, n);
       if (keep >= 16) *reinterpret_cast<uint4*>(a) = val;
-      else {
+      else {                                           // bytes behind the last token stay as they are
         const uint8_t* b = reinterpret_cast<const uint8_t*>(&val);
-        for (int y = 0; y < keep; ++y) a[y] = b[y];
+        for (int z = 0; z < keep; ++z) a[z] = b[z];
       }
     }
-    __syncthreads();
   }
 }
 // Page tables and lengths, behind the copies (which read the lengths): one block per item, a beam's column of entries at a time.
@@ -236,10 +239,7 @@ __global__ void __launch_bounds__(256) kv4_tables_kernel(int* __restrict__ pages
 inline bool aligned16(const void* p, const RowStrides& s, int elt) {
   return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(s.b * elt) | (uintptr_t)(s.t * elt) | (uintptr_t)(s.h * elt)) & 15) == 0;
 }
-inline unsigned grid_of(long long threads) {
-  const long long blocks = ceil_div_ll(threads, 256), most = (long long)sm_count() * 16;
-  return (unsigned)(blocks < most ? blocks : most);
-}
+inline unsigned at_most(long long blocks, long long most) { return (unsigned)(blocks < most ? blocks : most); }
 #define KV4_HEADS(HD_VALUE, CALL)                                                                          \
   switch (HD_VALUE) {                                                                                      \
     case 32: { constexpr int HD = 32; return CALL; }                                                       \
@@ -253,13 +253,18 @@ inline unsigned grid_of(long long threads) {
 template <typename T, int HD>
 int append(const Kv4Desc& d, int layer, const void* k, const void* v, const int* start, const int* counts, int n, RowStrides sk, RowStrides sv, cudaStream_t st) {
   constexpr int NB = HD / BLOCK, GROUP = NB <= 2 ? 4 : NB <= 4 ? 8 : 16;
-  const unsigned grid = grid_of((long long)d.slots * d.heads * n * GROUP);
+  const long long rows = (long long)d.slots * d.heads * n;
+  if (rows > 0x7fffffffLL - (1 << 20)) return LLMB_ERR_BAD_ARG;
+  const unsigned grid = at_most(ceil_div_ll(rows * GROUP, 256), (long long)sm_count() * 8);
   const bool vec = aligned16(k, sk, sizeof(T)) && aligned16(v, sv, sizeof(T));
   return launch_pdl(vec ? kv4_append_kernel<T, HD, true> : kv4_append_kernel<T, HD, false>, grid, 256, 0, st, d, layer, (const T*)k, (const T*)v, start, counts, n, sk, sv);
 }
 template <typename T, int HD>
 int values(const Kv4Desc& d, int layer, void* k, void* v, const int* start, const int* pages, int n, long long out_layer, RowStrides sk, RowStrides sv, cudaStream_t st) {
-  const unsigned grid = grid_of((long long)(layer < 0 ? d.layers : 1) * d.slots * n * d.heads * (HD / BLOCK));
+  const long long total = (long long)n * d.heads * (HD * (int)sizeof(T) / 16), planes = (long long)(layer < 0 ? d.layers : 1) * d.slots;
+  if (total > 0x7fffffffLL - (1 << 20) || planes > 0x7fffffffLL) return LLMB_ERR_BAD_ARG;
+  const unsigned gy = at_most(planes, 65535);
+  const dim3 grid(at_most(ceil_div_ll(total, 256), ceil_div_ll((long long)sm_count() * 16, gy)), gy);
   const bool vec = aligned16(k, sk, sizeof(T)) && aligned16(v, sv, sizeof(T)) && (out_layer * (int)sizeof(T)) % 16 == 0;
   return launch_pdl(vec ? kv4_values_kernel<T, HD, true> : kv4_values_kernel<T, HD, false>, grid, 256, 0, st, d, layer, (T*)k, (T*)v, start, pages, n, out_layer, sk, sv);
 }
@@ -292,7 +297,7 @@ LLMB_API int llmb_kv4_values(const Kv4Desc* d, const Kv4ValuesArgs* a, cudaStrea
 LLMB_API int llmb_kv4_reorder(const Kv4Desc* d, int* pages, int* lens, const int* parents, int K, cudaStream_t st) {
   const int items = K > 0 ? d->slots / K : 0;
   if (K < 1 || K > 64 || d->layers > 65535 || d->heads > 65535) return LLMB_ERR_BAD_ARG;
-  int rc = launch_pdl(kv4_reorder_kernel, dim3(items, d->heads, d->layers), REORDER_THREADS, 0, st, *d, (const int*)lens, parents, K);
+  int rc = launch_pdl(kv4_reorder_kernel, dim3(items, d->heads, d->layers), K <= 8 ? 256 : REORDER_PIECES / K / 32 * 32, 0, st, *d, (const int*)lens, parents, K);
   if (rc) return rc;
   return launch_pdl(kv4_tables_kernel, items, 256, 0, st, pages, lens, parents, K, d->capacity / PAGE, d->capacity);
 }
