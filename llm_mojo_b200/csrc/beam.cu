@@ -28,23 +28,30 @@ __device__ __forceinline__ unsigned long long ordered(double x) {
 // best first: the larger logit, then the lower column
 __device__ __forceinline__ unsigned long long key_of(float x, int col) { return (unsigned long long)ordered(x) << 32 | (uint32_t)~col; }
 
+// the largest of a warp's keys, to all lanes: the upper halves first, then the lower ones of those that have it
 __device__ __forceinline__ unsigned long long warp_max_u64(unsigned long long v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) { const unsigned long long w = __shfl_xor_sync(0xffffffffu, v, o); v = w > v ? w : v; }
-  return v;
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
+  return (unsigned long long)hi << 32 | lo;
 }
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
 // Workspace: stats [rows][chunks] float2 (maximum, sum of exponentials), lists [rows][chunks][K] of keys.
+//
+// The K-th largest of any 32 logits is no larger than the K-th largest of all.  Each warp takes that of its lanes' best, the block the largest
+// of them as a threshold; what is not below it (some forty of 4096) is ranked by counting.  Where more than CAND stay (ties, K > 32) the
+// list is taken from the registers one by one.
+constexpr int CAND = 512, RANKED = 192;
 template <typename T>
 __global__ void __launch_bounds__(THREADS) beam_chunk_kernel(float2* __restrict__ stats, unsigned long long* __restrict__ lists, const T* __restrict__ logits,
                                                              const bool* __restrict__ finished, int K, int V, long long ld, int chunks) {
   pdl_trigger();
   pdl_wait();
-  __shared__ unsigned long long cand[CHUNK];
-  __shared__ float red[THREADS / 32];
-  __shared__ uint32_t best_of[THREADS];
+  constexpr int WARPS = THREADS / 32;
+  __shared__ unsigned long long cand[CAND], best_of[WARPS];
+  __shared__ float red[WARPS];
+  __shared__ uint32_t level[WARPS];
   __shared__ int n_cand;
-  __shared__ uint32_t threshold;
   const int row = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   if (finished != nullptr && finished[row]) return;    // its one candidate does not depend on its logits
   const int c0 = chunk * CHUNK, w = min(CHUNK, V - c0);
@@ -52,91 +59,110 @@ __global__ void __launch_bounds__(THREADS) beam_chunk_kernel(float2* __restrict_
   float v[PER];
 #pragma unroll
   for (int j = 0; j < PER; ++j) { const int c = j * THREADS + tid; v[j] = c < w ? to_f<T>(x[c]) : -INFINITY; }
-  float m = -INFINITY;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) m = fmaxf(m, v[j]);
+  if (tid == 0) n_cand = 0;
+  float m = v[0];
   uint32_t mine = 0;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) if (j * THREADS + tid < w) mine = max(mine, ordered(v[j]));
-  best_of[tid] = mine;
-  m = warp_max(m);
-  if (lane == 0) red[warp] = m;
-  if (tid == 0) n_cand = 0;
+  for (int j = 1; j < PER; ++j) m = fmaxf(m, v[j]);
+  if (tid < w) mine = ordered(m);                      // a thread has columns if it has the first; a NaN counts -inf and is no maximum
+  const float wm = warp_max(m);
+  if (lane == 0) red[warp] = wm;
+  uint32_t t = 0;
+  if (K <= 32) {
+    uint32_t b = mine;
+    for (int i = 0; i < K; ++i) {
+      t = __reduce_max_sync(0xffffffffu, b);
+      if (lane == __ffs(__ballot_sync(0xffffffffu, b == t)) - 1) b = 0;
+    }
+  }
+  if (lane == 0) level[warp] = t;
   __syncthreads();
-  m = red[0];
+  m = red[0]; t = level[0];
 #pragma unroll
-  for (int i = 1; i < THREADS / 32; ++i) m = fmaxf(m, red[i]);
+  for (int i = 1; i < WARPS; ++i) { m = fmaxf(m, red[i]); t = max(t, level[i]); }
   float s = 0.f;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) if (j * THREADS + tid < w && !(v[j] == -INFINITY)) s += exp2f((v[j] - m) * 1.4426950408889634f);
+  for (int j = 0; j < PER; ++j) if (!(v[j] == -INFINITY)) s += ex2((v[j] - m) * 1.4426950408889634f);
   s = warp_sum(s);
+  unsigned above = 0;                                  // bit per element that stays
+#pragma unroll
+  for (int j = 0; j < PER; ++j) above |= (unsigned)(j * THREADS + tid < w && ordered(v[j]) >= t) << j;
+  if (above) {
+    int at = atomicAdd(&n_cand, __popc(above));        // any order: they are ranked below
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (above >> j & 1) { if (at < CAND) cand[at] = key_of(v[j], c0 + j * THREADS + tid); ++at; }
+  }
   __syncthreads();
   if (lane == 0) red[warp] = s;
-  // The K-th largest of the threads' best logits is no larger than the K-th largest of all: what is below it is out.
-  if (warp == 0) {
-    uint32_t b[THREADS / 32];
-#pragma unroll
-    for (int i = 0; i < THREADS / 32; ++i) b[i] = best_of[i * 32 + lane];
-    uint32_t t = 0;
-    for (int i = 0; i < K; ++i) {
-      uint32_t l = 0;
-#pragma unroll
-      for (int y = 0; y < THREADS / 32; ++y) l = max(l, b[y]);
-      t = __reduce_max_sync(0xffffffffu, l);
-      const unsigned has = __ballot_sync(0xffffffffu, l == t);
-      if (lane == __ffs(has) - 1) {
-        bool out = false;
-#pragma unroll
-        for (int y = 0; y < THREADS / 32; ++y) if (!out && b[y] == t) { b[y] = 0; out = true; }
-      }
+  const int n = n_cand;
+  unsigned long long* out = lists + ((long long)row * chunks + chunk) * K;
+  if (n <= RANKED) {
+    if (tid < n) {
+      const unsigned long long k = cand[tid];
+      int rank = 0;
+      for (int i = 0; i < n; ++i) rank += cand[i] > k;                   // keys differ from one another
+      if (rank < K) out[rank] = k;
     }
-    if (lane == 0) threshold = t;
-  }
-  __syncthreads();
-  const uint32_t t = threshold;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int c = j * THREADS + tid;
-    if (c < w && ordered(v[j]) >= t) cand[atomicAdd(&n_cand, 1)] = key_of(v[j], c0 + c);      // any order: they are sorted below
-  }
-  __syncthreads();
-  if (warp == 0) {
-    if (lane == 0) {
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < THREADS / 32; ++i) sum += red[i];
-      stats[(long long)row * chunks + chunk] = make_float2(m, sum);
-    }
-    const int n = n_cand;
-    unsigned long long* out = lists + ((long long)row * chunks + chunk) * K;
+    if (n + tid < K) out[n + tid] = 0;                 // fewer columns than K
+  } else {
     unsigned long long last = ~0ull;
-    for (int i = 0; i < K; ++i) {                      // keys differ from one another: the next one is the largest below the last
+    for (int i = 0; i < K; ++i) {                      // the largest key below the last
       unsigned long long b = 0;
-      for (int y = lane; y < n; y += 32) { const unsigned long long k = cand[y]; if (k < last && k > b) b = k; }
-      last = warp_max_u64(b);
-      if (lane == 0) out[i] = last;                    // 0 where the chunk has fewer than K columns
-      if (last == 0) { for (int y = i + 1; y < K; ++y) if (lane == 0) out[y] = 0; break; }
+      if (n <= CAND) {
+        for (int y = tid; y < n; y += THREADS) { const unsigned long long k = cand[y]; if (k < last && k > b) b = k; }
+      } else {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          if (above >> j & 1) { const unsigned long long k = key_of(v[j], c0 + j * THREADS + tid); if (k < last && k > b) b = k; }
+      }
+      b = warp_max_u64(b);
+      if (lane == 0) best_of[warp] = b;
+      __syncthreads();
+      last = best_of[0];
+#pragma unroll
+      for (int y = 1; y < WARPS; ++y) last = best_of[y] > last ? best_of[y] : last;
+      if (tid == 0) out[i] = last;                     // 0 where the chunk has fewer than K columns; nothing is below 0
+      __syncthreads();
     }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) sum += red[i];
+    stats[(long long)row * chunks + chunk] = make_float2(m, sum);
   }
 }
 
+// One block per item.  Its warps add up the log-sum-exps; then one warp merges the sorted lists by their heads, whose values it keeps in shared
+// memory; the lists come along where they fit (`staged`).  A beam that is not alive has one list of its own making in the place of its
+// first chunk's.
 __global__ void __launch_bounds__(THREADS) beam_merge_kernel(float* __restrict__ scores_out, int* __restrict__ tokens, int* __restrict__ parents,
                                                              bool* __restrict__ finished_out, const float* __restrict__ scores, const bool* __restrict__ finished,
-                                                             const float2* __restrict__ stats, const unsigned long long* __restrict__ lists, int K, int V, int eos, int chunks) {
+                                                             const float2* __restrict__ stats, const unsigned long long* __restrict__ lists, int K, int V, int eos, int chunks,
+                                                             int staged) {
   pdl_trigger();
   pdl_wait();
-  extern __shared__ int heads[];                       // [K * chunks] next entry of each list
+  extern __shared__ unsigned long long sm[];
   __shared__ double lse[BEAM_MAX];
+  __shared__ float score[BEAM_MAX];
   __shared__ int kind[BEAM_MAX];                       // 0: alive, 1: finished, 2: offers nothing
-  __shared__ float out_score[BEAM_MAX];
-  const int item = blockIdx.x, tid = threadIdx.x, lane = tid % 32;
+  __shared__ bool fin[BEAM_MAX];
+  const int item = blockIdx.x, tid = threadIdx.x, lane = tid % 32, n_lists = K * chunks;
+  unsigned long long* const value = sm;                // [n_lists] ordered value of each list's head, 0: none left
+  uint32_t* const flat = reinterpret_cast<uint32_t*>(sm + n_lists);      // its k V + v
+  int* const next = reinterpret_cast<int*>(flat + n_lists);              // the entry behind it
+  unsigned long long* const stage = sm + 2 * n_lists;
+  const unsigned long long* mine = lists + (long long)item * n_lists * K;
+  if (staged) for (int i = tid; i < n_lists * K; i += THREADS) stage[i] = mine[i];
   for (int k = tid / 32; k < K; k += THREADS / 32) {
     const long long row = (long long)item * K + k;
     const float sc = scores[row];
-    const bool fin = finished != nullptr && finished[row], ok = fabsf(sc) <= 3.402823466e38f;
+    const bool f = finished != nullptr && finished[row], ok = fabsf(sc) <= 3.402823466e38f;
     float m = -INFINITY;
     double sum = 0.0;
-    if (!fin) {
+    if (!f) {
       for (int c = lane; c < chunks; c += 32) m = fmaxf(m, stats[row * chunks + c].x);
       m = warp_max(m);
       for (int c = lane; c < chunks; c += 32) {
@@ -148,52 +174,48 @@ __global__ void __launch_bounds__(THREADS) beam_merge_kernel(float* __restrict__
     }
     if (lane == 0) {
       const double l = (double)m + log(sum);
-      lse[k] = l;
-      kind[k] = !ok ? 2 : fin ? 1 : l - l == 0.0 ? 0 : 2;
+      lse[k] = l; score[k] = sc; fin[k] = f;
+      kind[k] = !ok ? 2 : f ? 1 : l - l == 0.0 ? 0 : 2;
     }
   }
-  for (int i = tid; i < K * chunks; i += THREADS) heads[i] = 0;
+  __syncthreads();
+  // entry e of list l becomes its head
+  auto advance = [&](int l, int e) {
+    const int k = l / chunks, kd = kind[k];
+    unsigned long long val = 0;
+    int col = 0;
+    if (e < K) {
+      if (kd == 0) {
+        const unsigned long long x = staged ? stage[l * K + e] : mine[(long long)l * K + e];
+        if (x != 0) { col = (int)~(uint32_t)x; val = ordered((double)score[k] + ((double)unordered((uint32_t)(x >> 32)) - lse[k]) + 0.0); }
+      } else if (l == k * chunks) {                    // finished: eos first; then, or if it offers nothing, the others, all at -inf
+        col = kd == 2 ? e : e == 0 ? eos : e - 1 < eos ? e - 1 : e;
+        val = ordered(kd == 1 && e == 0 ? (double)score[k] + 0.0 : (double)-INFINITY);
+      }
+    }
+    value[l] = val; flat[l] = (uint32_t)k * (uint32_t)V + (uint32_t)col; next[l] = e + 1;
+  };
+  for (int l = tid; l < n_lists; l += THREADS) advance(l, 0);
   __syncthreads();
   if (tid >= 32) return;
-  // The lists' heads, one after another; a beam that is not alive has one list of its own making in the place of its first chunk's.
   for (int i = 0; i < K; ++i) {
-    unsigned long long bk = 0;                         // of the best head: its ordered value, its flat index, its list
+    unsigned long long bk = 0;
     uint32_t bi = 0xffffffffu;
     int bl = -1;
-    for (int l = lane; l < K * chunks; l += 32) {
-      const int k = l / chunks, h = heads[l], kd = kind[k];
-      const long long row = (long long)item * K + k;
-      double val = -INFINITY;
-      int col;
-      if (h >= K) continue;
-      if (kd == 0) {
-        const unsigned long long e = lists[(row * chunks + l % chunks) * K + h];
-        if (e == 0) continue;
-        col = (int)~(uint32_t)e;
-        val = (double)scores[row] + ((double)unordered((uint32_t)(e >> 32)) - lse[k]);
-      } else {
-        if (l % chunks != 0) continue;
-        if (kd == 1) {                                 // eos first, then the others, which are all at -inf
-          col = h == 0 ? eos : h - 1 < eos ? h - 1 : h;
-          if (h == 0) val = (double)scores[row];
-        } else col = h;
-      }
-      const unsigned long long key = ordered(val + 0.0);
-      const uint32_t idx = (uint32_t)k * (uint32_t)V + (uint32_t)col;
-      if (key > bk || (key == bk && idx < bi)) { bk = key; bi = idx; bl = l; }
+    for (int l = lane; l < n_lists; l += 32) {
+      const unsigned long long x = value[l];
+      if (x > bk || (x == bk && x != 0 && flat[l] < bi)) { bk = x; bi = flat[l]; bl = l; }
     }
     const unsigned long long top = warp_max_u64(bk);
     const uint32_t idx = __reduce_min_sync(0xffffffffu, bk == top ? bi : 0xffffffffu);
     if (bl >= 0 && bk == top && bi == idx) {           // one lane: flat indexes differ
-      heads[bl] += 1;
-      const int k = (int)(idx / (uint32_t)V), tok = (int)(idx % (uint32_t)V);
-      const unsigned long long b = top >> 63 ? top ^ (1ull << 63) : ~top;
+      const int k = (int)(idx / (uint32_t)V), tok = (int)(idx - (uint32_t)k * (uint32_t)V);
       const long long at = (long long)item * K + i;
-      out_score[i] = (float)__longlong_as_double((long long)b);
-      scores_out[at] = out_score[i];
+      scores_out[at] = (float)__longlong_as_double((long long)(top >> 63 ? top ^ (1ull << 63) : ~top));
       tokens[at] = tok;
       parents[at] = k;
-      if (finished_out != nullptr) finished_out[at] = tok == eos || kind[k] == 1 || (finished != nullptr && finished[(long long)item * K + k]);
+      if (finished_out != nullptr) finished_out[at] = tok == eos || fin[k];
+      advance(bl, next[bl]);
     }
     __syncwarp();
   }
@@ -211,7 +233,7 @@ struct BeamSelectArgs {
 
 LLMB_API int llmb_beam_select(const BeamSelectArgs* a, cudaStream_t st) {
   const int K = a->K, V = a->V, chunks = ceil_div(V, CHUNK), rows = a->B * K;
-  if (K < 1 || K > BEAM_MAX || rows > 65535 || (long long)K * chunks * 4 > 40 * 1024) return LLMB_ERR_BAD_ARG;
+  if (K < 1 || K > BEAM_MAX || rows > 65535 || (long long)K * chunks * 16 > 46 * 1024) return LLMB_ERR_BAD_ARG;
   float2* stats = (float2*)a->work;
   unsigned long long* lists = (unsigned long long*)(stats + (long long)rows * chunks);
   const dim3 grid(chunks, rows);
@@ -219,6 +241,8 @@ LLMB_API int llmb_beam_select(const BeamSelectArgs* a, cudaStream_t st) {
                ? launch_pdl(beam_chunk_kernel<__nv_bfloat16>, grid, THREADS, 0, st, stats, lists, (const __nv_bfloat16*)a->logits, a->finished, K, V, a->ld, chunks)
                : launch_pdl(beam_chunk_kernel<float>, grid, THREADS, 0, st, stats, lists, (const float*)a->logits, a->finished, K, V, a->ld, chunks);
   if (rc) return rc;
-  return launch_pdl(beam_merge_kernel, a->B, THREADS, (size_t)K * chunks * 4, st, a->scores_out, a->tokens, a->parents, a->finished_out, a->scores, a->finished,
-                    (const float2*)stats, (const unsigned long long*)lists, K, V, a->eos, chunks);
+  const size_t heads = (size_t)K * chunks * 16, staged = (size_t)K * chunks * K * 8;
+  const bool stage = heads + staged <= 48 * 1024 - 2048;                 // what a block may have without asking
+  return launch_pdl(beam_merge_kernel, a->B, THREADS, stage ? heads + staged : heads, st, a->scores_out, a->tokens, a->parents, a->finished_out, a->scores, a->finished,
+                    (const float2*)stats, (const unsigned long long*)lists, K, V, a->eos, chunks, (int)stage);
 }

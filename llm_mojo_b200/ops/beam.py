@@ -41,8 +41,8 @@ def beam_select(scores_out: torch.Tensor, tokens: torch.Tensor, parents: torch.T
         raise ValueError(f"1 to {BEAM_MAX} beams, not {K}")
     if not K <= vocab_size <= rows[1] or K * vocab_size >= 2 ** 31:
         raise ValueError(f"vocabulary of {vocab_size}: at least {K} beams, at most the {rows[1]} columns, and K x V below 2^31")
-    if B * K > 65535 or K * -(-vocab_size // 4096) > 10240:
-        raise ValueError(f"{B} items of {K} beams over {vocab_size} tokens are too many: at most 65535 rows, and K x V up to 40 million")
+    if B * K > 65535 or K * -(-vocab_size // 4096) > 2944:
+        raise ValueError(f"{B} items of {K} beams over {vocab_size} tokens are too many: at most 65535 rows, and K x V up to 12 million")
     if not -1 <= eos < vocab_size:
         raise ValueError(f"eos {eos} is no token of a vocabulary of {vocab_size}")
     if finished is not None and eos < 0:

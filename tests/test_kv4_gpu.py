@@ -108,6 +108,25 @@ def test_append_of_midpoints_extremes_and_odd_addresses():
         assert torch.equal(ko.double(), want) and torch.equal(vo.double(), -want)
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("unit", [2.0 ** -32, UNIT, 1.0, 2.0 ** 20])
+def test_append_with_every_scale(dtype, unit):
+    """Every scale with every midpoint between two levels, exact and (fp32) with its neighbours; rows that are not finite."""
+    level = torch.tensor([6.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, -6.0, -0.25, -0.75, -1.25, -1.75, -2.5, -3.5, -5.0], dtype=torch.float64, device=DEV)
+    scale = torch.arange(1, 127, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn).double()
+    exact = (scale.view(-1, 1) * level).mul(unit).float()                    # [126, 16]: three bits times four
+    x = torch.stack([exact, exact if dtype == BF else torch.nextafter(exact, exact * 2), exact if dtype == BF else torch.nextafter(exact, exact * 0)], 1)
+    x = torch.cat([x.reshape(1, -1, 1, 16), torch.full((1, 6, 1, 16), 1e38, device=DEV) * level.float()], 1).to(dtype)
+    x = x.reshape(1, -1, 1, 64)
+    c = ops.KV4Cache(*(torch.zeros(1, 1, 1, 128, w, dtype=torch.uint8, device=DEV) for w in (32, 4, 32, 4)), k_unit=unit, v_unit=unit * 2)
+    ops.kv4_append(c, 0, x, x * 2 if unit < 1e6 else x, i32([0]))
+    ko, vo = (torch.empty(x.shape, device=DEV) for _ in range(2))
+    ops.kv4_values(ko, vo, c, 0, i32([0]))
+    want = rounded64(x.nan_to_num(0.0, 0.0, 0.0), unit)
+    want[~torch.isfinite(x).all(-1)] = math.nan              # 6e38 is infinite
+    assert torch.equal(ko.double().nan_to_num(7e7), want.nan_to_num(7e7))
+
+
 def test_positions_before_the_cache_and_bad_pages():
     c, d = filled(2, 2, 64, [64, 64], 128)
     x = rnd(2, 4, 2, 64, dtype=BF, seed=9)
