@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(THREADS) beam_chunk_kernel(float2* __restrict_
   uint32_t mine = 0;
 #pragma unroll
   for (int j = 1; j < PER; ++j) m = fmaxf(m, v[j]);
-  if (tid < w) mine = ordered(m);                      // a thread has columns if it has the first; a NaN counts -inf and is no maximum
+  if (tid < w) mine = ordered(m);                      // a thread has columns if it has the first
   const float wm = warp_max(m);
   if (lane == 0) red[warp] = wm;
   uint32_t t = 0;
@@ -80,18 +80,26 @@ __global__ void __launch_bounds__(THREADS) beam_chunk_kernel(float2* __restrict_
   m = red[0]; t = level[0];
 #pragma unroll
   for (int i = 1; i < WARPS; ++i) { m = fmaxf(m, red[i]); t = max(t, level[i]); }
+  const float safe = m == -INFINITY ? 0.f : m, level_f = unordered(t);
   float s = 0.f;
+  unsigned above = 0;                                  // bit per element that stays; a NaN may go, its beam offers nothing
 #pragma unroll
-  for (int j = 0; j < PER; ++j) if (!(v[j] == -INFINITY)) s += ex2((v[j] - m) * 1.4426950408889634f);
+  for (int j = 0; j < PER; ++j) {
+    s += ex2((v[j] - safe) * 1.4426950408889634f);
+    above |= (unsigned)(v[j] >= level_f) << j;
+  }
+  if (K > 32) above = 0xffffffffu;
+  above &= tid < w ? (2u << (w - 1 - tid) / THREADS) - 1 : 0u;           // columns that there are
   s = warp_sum(s);
-  unsigned above = 0;                                  // bit per element that stays
-#pragma unroll
-  for (int j = 0; j < PER; ++j) above |= (unsigned)(j * THREADS + tid < w && ordered(v[j]) >= t) << j;
+  const unsigned kept = above;
   if (above) {
     int at = atomicAdd(&n_cand, __popc(above));        // any order: they are ranked below
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (above >> j & 1) { if (at < CAND) cand[at] = key_of(v[j], c0 + j * THREADS + tid); ++at; }
+    while (above) {                                    // mostly one, read again
+      const int c = (__ffs(above) - 1) * THREADS + tid;
+      above &= above - 1;
+      if (at < CAND) cand[at] = key_of(to_f<T>(x[c]), c0 + c);
+      ++at;
+    }
   }
   __syncthreads();
   if (lane == 0) red[warp] = s;
@@ -114,7 +122,7 @@ __global__ void __launch_bounds__(THREADS) beam_chunk_kernel(float2* __restrict_
       } else {
 #pragma unroll
         for (int j = 0; j < PER; ++j)
-          if (above >> j & 1) { const unsigned long long k = key_of(v[j], c0 + j * THREADS + tid); if (k < last && k > b) b = k; }
+          if (kept >> j & 1) { const unsigned long long k = key_of(v[j], c0 + j * THREADS + tid); if (k < last && k > b) b = k; }
       }
       b = warp_max_u64(b);
       if (lane == 0) best_of[warp] = b;

@@ -200,22 +200,39 @@ __device__ __forceinline__ int parent_of(const int* parents, int item, int j, in
 }
 __device__ __forceinline__ int length_of(const int* lens, int slot, int capacity) { return min(max(lens[slot], 0), capacity); }
 
+struct Kv4Page { long long codes, scales; int tokens, source; };      // offsets in bytes, tokens in use, and for a copy the beam it is of
 // The page that is being filled: its used part is contiguous in each of the four tensors.  A thread takes the same 16 bytes of every beam's page
 // that is somebody's parent into a column of shared memory of its own, then gives every beam with another parent its parent's.  So no
 // thread waits for another, and everything is read before it is written: other threads write other bytes.  Blocks share an item's heads and layers.
-__global__ void __launch_bounds__(128) kv4_reorder_kernel(const Kv4Desc d, const int* __restrict__ lens, const int* __restrict__ parents, int K) {
+__global__ void __launch_bounds__(128, 12) kv4_reorder_kernel(const Kv4Desc d, const int* __restrict__ lens, const int* __restrict__ parents, int K) {
   pdl_trigger();
   pdl_wait();
-  extern __shared__ uint4 buf[];                       // a piece of each beam for every thread
-  __shared__ int of[64], len[64], wanted[64], longest;
-  const int item = blockIdx.x, j0 = threadIdx.x;
-  for (int j = j0; j < K; j += blockDim.x) { of[j] = parent_of(parents, item, j, K); len[j] = length_of(lens, item * K + j, d.capacity); wanted[j] = 0; }
-  if (j0 == 0) longest = 0;
-  __syncthreads();
-  for (int j = j0; j < K; j += blockDim.x)
-    if (of[j] != j && len[of[j]] % PAGE) { wanted[of[j]] = 1; atomicMax(&longest, len[of[j]] % PAGE); }
-  __syncthreads();
+  extern __shared__ uint4 buf[];                       // a piece of each source for every thread
+  __shared__ Kv4Page from[64], to[64];                 // the pages that are read, and those that are written
+  __shared__ int place_of[64], n_from, n_to, longest;
+  const int item = blockIdx.x;
   const int cb = d.head_size / 2, sb = d.head_size / BLOCK;
+  if (threadIdx.x == 0) n_from = n_to = longest = 0;
+  for (int j = threadIdx.x; j < K; j += blockDim.x) place_of[j] = -1;
+  __syncthreads();
+  auto page_of = [&](int j, int n) {                   // where beam j keeps the page in which n tokens end, from the item's first slot on
+    const long long before = (long long)(n / PAGE) * PAGE;
+    return Kv4Page{j * d.code_slot + before * cb, j * d.scale_slot + before * sb, n % PAGE, 0};
+  };
+  for (int j = threadIdx.x; j < K; j += blockDim.x) {
+    const int p = parent_of(parents, item, j, K), n = length_of(lens, item * K + p, d.capacity);
+    if (p == j || n % PAGE == 0) continue;
+    if (atomicCAS(&place_of[p], -1, -2) == -1) {       // the first to name this parent
+      const int i = atomicAdd(&n_from, 1);
+      from[i] = page_of(p, n);
+      atomicExch(&place_of[p], i);
+    }
+    Kv4Page w = page_of(j, n);
+    w.source = p;
+    to[atomicAdd(&n_to, 1)] = w;
+    atomicMax(&longest, n % PAGE);
+  }
+  __syncthreads();
   const unsigned code_pieces = ceil_div(longest * cb, 16), scale_pieces = ceil_div(longest * sb, 16), half = code_pieces + scale_pieces;
   const unsigned all = d.layers * d.heads * 2 * half;
   for (unsigned x = blockIdx.y * blockDim.x + threadIdx.x; x < all; x += gridDim.y * blockDim.x) {
@@ -225,23 +242,18 @@ __global__ void __launch_bounds__(128) kv4_reorder_kernel(const Kv4Desc d, const
     if (is_v) y -= half;
     const bool is_scale = y >= code_pieces;
     const int bytes = is_scale ? sb : cb, first = (is_scale ? y - code_pieces : y) * 16;           // bytes of a token; the piece's first byte
-    const long long slot_stride = is_scale ? d.scale_slot : d.code_slot;
-    uint8_t* const base = (is_scale ? (is_v ? d.vs : d.ks) + layer * d.scale_layer : (is_v ? d.vc : d.kc) + layer * d.code_layer) +
-                          item * K * slot_stride + (long long)h * d.capacity * bytes + first;
-    auto place = [&](int j, int n) { return base + j * slot_stride + (long long)(n / PAGE) * PAGE * bytes; };
-    for (int j = 0; j < K; j += 4) {                   // four loads in flight
-      uint4 v[4];
-#pragma unroll
-      for (int z = 0; z < 4; ++z)
-        if (j + z < K && wanted[j + z] && first < (len[j + z] % PAGE) * bytes) v[z] = *reinterpret_cast<const uint4*>(place(j + z, len[j + z]));
-#pragma unroll
-      for (int z = 0; z < 4; ++z) if (j + z < K) buf[(j + z) * blockDim.x + threadIdx.x] = v[z];
-    }
-    for (int j = 0; j < K; ++j) {
-      const int p = of[j], n = len[p], keep = (n % PAGE) * bytes - first;
-      if (p == j || keep <= 0) continue;
-      const uint4 val = buf[p * blockDim.x + threadIdx.x];
-      uint8_t* const a = place(j, n);
+    uint8_t* const base = (is_scale ? (is_v ? d.vs : d.ks) + layer * d.scale_layer + item * K * d.scale_slot
+                                    : (is_v ? d.vc : d.kc) + layer * d.code_layer + item * K * d.code_slot) + (long long)h * d.capacity * bytes + first;
+    for (int j = 0; j < n_from; ++j)                   // asynchronous copies: all of them are in flight at once
+      if (first < from[j].tokens * bytes)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(&buf[j * blockDim.x + threadIdx.x])),
+                     "l"(base + (is_scale ? from[j].scales : from[j].codes)) : "memory");
+    asm volatile("cp.async.wait_all;" ::: "memory");   // a thread reads nothing but its own copies
+    for (int j = 0; j < n_to; ++j) {
+      const int keep = to[j].tokens * bytes - first;
+      if (keep <= 0) continue;
+      const uint4 val = buf[place_of[to[j].source] * blockDim.x + threadIdx.x];
+      uint8_t* const a = base + (is_scale ? to[j].scales : to[j].codes);
       if (keep >= 16) *reinterpret_cast<uint4*>(a) = val;
       else {                                           // bytes behind the last token stay as they are
         const uint8_t* b = reinterpret_cast<const uint8_t*>(&val);
