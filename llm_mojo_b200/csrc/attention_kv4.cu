@@ -12,17 +12,6 @@ using namespace kv4;
 namespace cg = cooperative_groups;
 
 namespace {
-struct Kv4Attn {
-  Kv4Desc d;
-  void* out; const void* q;
-  const int *lens, *counts, *pages;
-  int layer, n, group, splits;
-  float scale_log2;
-  long long qb, qt, qh, ob, ot, oh;                    // element strides
-  int* status;
-  bool q_vec;                                          // rows of q can be read 16 bytes at a time
-};
-
 // The products are taken transposed, S^T = K q^T and o^T = V^T P^T (mma.sync m16n8k16, f16 operands, fp32 sums): 16 keys fill a tile's rows
 // and eight columns are rows of q, so that a single query pads to 8 and not to 128 (as it would in a tcgen05 product), and the codes
 // go from shared memory to registers straight into operands:
@@ -507,9 +496,11 @@ int run_mma(Kv4Attn p, cudaStream_t st) {
   const int warps = log_w == 3 ? 8 : 4;
   return launch_pdl_cluster(dim3(p.splits), kernel, dim3((unsigned)(ceil_div_ll(units << log_w, warps) * p.splits)), warps * 32, warps * S::SMEM_WARP, st, p, log_w, (int)tiles);
 }
+constexpr int PROMPT_ROWS = 64;
 template <typename T, int HD>
 int run(const Kv4Attn& p, cudaStream_t st) {
   const long long rows = (long long)p.n * p.group;
+  if (sizeof(T) == 2 && HD == 64 && rows >= PROMPT_ROWS) return kv4_attention_prompt(p, st);
   constexpr int R8 = sizeof(T) == 4 ? 4 : 8, MOST = HD <= 64 ? 4 : 2;
   if (rows <= R8 / 2) return run_mma<T, HD, 1, true>(p, st);
   if (rows <= R8) return run_mma<T, HD, 1, false>(p, st);

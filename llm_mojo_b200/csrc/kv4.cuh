@@ -50,3 +50,18 @@ __device__ __forceinline__ float2 f16x2_f32(uint32_t h) {
 }
 __device__ __forceinline__ float e4m3_f32(uint32_t byte) { return f16x2_f32(e4m3x2_f16x2(byte)).x; }
 }  // namespace kv4
+
+// One call of the attention over a cache.
+struct Kv4Attn {
+  Kv4Desc d;
+  void* out; const void* q;
+  const int *lens, *counts, *pages;
+  int layer, n, group, splits;
+  float scale_log2;
+  long long qb, qt, qh, ob, ot, oh;                    // element strides
+  int* status;
+  bool q_vec;                                          // rows of q can be read 16 bytes at a time
+};
+
+// Rows of at least KV4_PROMPT_ROWS on the tcgen05 kernel (bf16, heads of 64): attention_kv4_prompt.cu
+int kv4_attention_prompt(const Kv4Attn& p, cudaStream_t st);
