@@ -15,8 +15,9 @@ using namespace kv4;
 
 namespace {
 constexpr int KP_NS = 3;                                  // K/V ring depth (32 KB per stage)
+constexpr int KP_RAW = 3, RAW_BYTES = 128 * 36;           // blocks of codes and scales on their way, per operand
 constexpr int KP_THREADS = 512;
-constexpr int KP_SMEM = 4 * T128 /*Q: 2 buffers x 2 tiles*/ + KP_NS * 2 * T128 /*K,V ring*/ + 1024 /*alignment*/ + 512 /*barriers*/ +
+constexpr int KP_SMEM = 4 * T128 /*Q: 2 buffers x 2 tiles*/ + KP_NS * 2 * T128 /*K,V ring*/ + 2 * KP_RAW * RAW_BYTES /*codes and scales*/ + 1024 /*alignment*/ + 512 /*barriers*/ +
                         4096 /*row statistics*/ + 2048 /*row factors*/;
 constexpr uint32_t IDESC_QK = make_idesc(FMT_F16, FMT_F16, 0, 0, 128, 128);
 constexpr uint32_t IDESC_PV = make_idesc(FMT_F16, FMT_F16, 0, 1, 128, 64);     // A (P) K-major from TMEM, B (V) stored [keys, HS]
@@ -70,7 +71,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) attention_kv4_prompt_kernel(con
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* sQ = sm;                                 // buffer qb: tile t0 at qb*2*T128, tile t0+1 at +T128
   unsigned char* sKV = sQ + 4 * T128;                     // stage s: K block at s*2*T128, V block at +T128
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + KP_NS * 2 * T128);
+  unsigned char* sRaw = sKV + KP_NS * 2 * T128;           // keys' blocks, then values': codes of 128 tokens, then scales
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sRaw + 2 * KP_RAW * RAW_BYTES);
   uint64_t* q_full = bars;                                // [2] the output warpgroup's four warps
   uint64_t* q_empty = q_full + 2;                         // [lane][2] the lane's last score product of the item is complete
   uint64_t* kv_full = q_empty + 4;                        // [NS] the two warps that write K and V
@@ -81,7 +83,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) attention_kv4_prompt_kernel(con
   uint64_t* pv_done = p_full + 2;                         // [2] per lane: O += P V complete (P may be overwritten)
   uint64_t* o_free = pv_done + 2;                         // [2] per lane: the item's output has left TMEM
   uint64_t* fin = o_free + 2;                             // [2] per lane: the item's row statistics are in shared memory
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fin + 2);
+  uint64_t* raw_full = fin + 2;                           // [2][RAW] a block's codes and scales are in shared memory
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_full + 2 * KP_RAW);
   float* stats = reinterpret_cast<float*>(bars + 64);     // [lane][item parity][l][128 rows] (m is not needed)
   float* factor = stats + 1024;                           // [qb][tile][128 rows]: products to log2 units
 
@@ -92,6 +95,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) attention_kv4_prompt_kernel(con
       mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); mbar_init(&p_full[i], 4);
       mbar_init(&pv_done[i], 1); mbar_init(&o_free[i], 4); mbar_init(&fin[i], 4);
     }
+    for (int i = 0; i < 2 * KP_RAW; ++i) mbar_init(&raw_full[i], 1);
     for (int i = 0; i < KP_NS; ++i) { mbar_init(&kv_full[i], 2); mbar_init(&kv_empty[i], 1); mbar_init(&kv_empty[KP_NS + i], 1); }
     fence_barrier_init();
   }
@@ -108,52 +112,64 @@ __global__ void __launch_bounds__(KP_THREADS, 1) attention_kv4_prompt_kernel(con
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     if (warp == 12 || warp == 15) {
       // ---------------------------------------------------------- keys (warp 12) and values (warp 15) into the ring
-      // A lane takes 16 bytes of codes, half a row, of eight rows; the block's loads are issued one block ahead, before the wait for its stage.
+      // Untiled bulk copies bring a block's codes and scales (contiguous within a page) into a ring of the warp's own, three blocks ahead of their
+      // conversion; held in registers instead, they were spilled, and every block waited for its loads (145 us where this takes REPLACE).
       const bool is_v = warp == 15;
       const uint8_t* codes = (is_v ? p.d.vc : p.d.kc) + p.layer * p.d.code_layer;
       const uint8_t* scales = (is_v ? p.d.vs : p.d.ks) + p.layer * p.d.scale_layer;
-      const int half = lane & 1, key0 = lane >> 1;        // rows key0 + 16 x
+      unsigned char* raw = sRaw + (is_v ? KP_RAW * RAW_BYTES : 0);
+      uint64_t* full = raw_full + (is_v ? KP_RAW : 0);
+      const int half = lane & 1, key0 = lane >> 1;        // a lane takes half a row, 16 bytes of codes, of the rows key0 + 16 x
       KpItem it = kp_item(p, grid, 0);
-      int k = 0, j = 0;
-      uint4 w[8]; uint32_t f[8];
-      auto settle = [&]() { while (it.valid && j >= it.most) { j = 0; it = kp_item(p, grid, ++k); } };
-      auto load = [&]() {
-        const int base = j * TILE;
-        int slot[2]; bool bad[2];
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          slot[y] = it.s;
-          const int page = base / PAGE + y;
-          if (p.pages && page < p.d.capacity / PAGE) slot[y] = p.pages[(long long)it.s * (p.d.capacity / PAGE) + page];
-          bad[y] = slot[y] < 0 || slot[y] >= p.d.slots;
-          if (bad[y]) slot[y] = it.s;
+      int k = 0, j = 0, issued = 0;
+      uint32_t state = 0;                                 // four bits per stage: page 0 / 1 names no slot, page 1 lies behind the cache
+      auto issue = [&]() {
+        while (it.valid && j >= it.most) { j = 0; it = kp_item(p, grid, ++k); }
+        if (!it.valid) return;
+        const int st = issued % KP_RAW, page0 = 2 * j, pages = p.d.capacity / PAGE;
+        const bool two = page0 + 1 < pages;
+        int s0 = it.s, s1 = it.s;
+        if (p.pages) {
+          s0 = p.pages[(long long)it.s * pages + page0];
+          if (two) s1 = p.pages[(long long)it.s * pages + page0 + 1];
         }
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const int key = base + key0 + 16 * x, y = x / 4;
-          w[x] = make_uint4(0, 0, 0, 0); f[x] = 0;
-          if (key < p.d.capacity) {                       // the last block of an odd number of pages reaches beyond the cache
-            const long long row = (long long)it.h * p.d.capacity + key;
-            w[x] = *reinterpret_cast<const uint4*>(codes + slot[y] * p.d.code_slot + row * 32 + half * 16);
-            f[x] = *reinterpret_cast<const uint16_t*>(scales + slot[y] * p.d.scale_slot + row * 4 + half * 2);
-            if (bad[y]) f[x] = 0x7f7f;                    // NaN for whoever sees the page
+        const bool b0 = s0 < 0 || s0 >= p.d.slots, b1 = s1 < 0 || s1 >= p.d.slots;
+        if (b0) s0 = it.s;
+        if (b1) s1 = it.s;
+        state = (state & ~(15u << (4 * st))) | (uint32_t)(b0 | b1 << 1 | !two << 2) << (4 * st);
+        if (lane == 0) {
+          const long long at = (long long)it.h * pages + page0;
+          unsigned char* dst = raw + st * RAW_BYTES;
+          mbar_expect_tx(&full[st], two ? RAW_BYTES : RAW_BYTES / 2);
+          bulk_load_1d(dst, codes + s0 * p.d.code_slot + at * PAGE * 32, PAGE * 32, &full[st]);
+          bulk_load_1d(dst + 2 * PAGE * 32, scales + s0 * p.d.scale_slot + at * PAGE * 4, PAGE * 4, &full[st]);
+          if (two) {
+            bulk_load_1d(dst + PAGE * 32, codes + s1 * p.d.code_slot + (at + 1) * PAGE * 32, PAGE * 32, &full[st]);
+            bulk_load_1d(dst + 2 * PAGE * 32 + PAGE * 4, scales + s1 * p.d.scale_slot + (at + 1) * PAGE * 4, PAGE * 4, &full[st]);
           }
         }
+        ++j; ++issued;
       };
-      settle();
-      if (it.valid) load();
-      for (int g = 0; it.valid && !failed; ++g) {
-        const int st = g % KP_NS;
+      for (int x = 0; x < KP_RAW; ++x) issue();
+      for (int g = 0; g < issued && !failed; ++g) {
+        const int st = g % KP_NS, rs = g % KP_RAW;
+        if (!mbar_wait(&full[rs], (g / KP_RAW) & 1)) { KP_FAIL(); break; }
         if (g >= KP_NS && !(mbar_wait(&kv_empty[st], ((g / KP_NS) + 1) & 1) && mbar_wait(&kv_empty[KP_NS + st], ((g / KP_NS) + 1) & 1))) { KP_FAIL(); break; }
         unsigned char* tile = sKV + st * 2 * T128 + (is_v ? T128 : 0);
-#pragma unroll
+        const unsigned char* src = raw + rs * RAW_BYTES;
+        const uint32_t how = state >> (4 * rs);
+#pragma unroll 4
         for (int x = 0; x < 8; ++x) {
           const int row = key0 + 16 * x;
-          uint32_t two = e4m3x2_f16x2(f[x]);
+          const uint4 w = *reinterpret_cast<const uint4*>(src + row * 32 + half * 16);
+          uint32_t f = *reinterpret_cast<const uint16_t*>(src + 2 * PAGE * 32 + row * 4 + half * 2);
+          if (x >= 4 && (how & 4)) f = 0;                 // behind the cache: whatever lies there, times 0
+          if (how & (x < 4 ? 1 : 2)) f = 0x7f7f;          // NaN for whoever sees the page
+          uint32_t two = e4m3x2_f16x2(f);
           // A NaN scale of a value becomes 448: the key's scales are NaN as well and say so to the rows that see it, and to no other.
           if (is_v) asm("min.f16x2 %0, %0, %1;" : "+r"(two) : "r"(0x5f005f00u));
           const uint32_t s0 = __byte_perm(two, two, 0x1010), s1 = __byte_perm(two, two, 0x3232);
-          const uint32_t word[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
+          const uint32_t word[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
             uint32_t h[4];
@@ -164,12 +180,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) attention_kv4_prompt_kernel(con
           }
         }
         fence_proxy_async();
-        __syncwarp();
+        __syncwarp();                                     // every lane has read the raw stage, too
         if (lane == 0) mbar_arrive(&kv_full[st]);
-        ++j;
-        settle();
-        if (it.valid) load();
+        issue();
       }
+      if (failed)                                         // leave with no copy in flight
+        for (int x = 0; x < KP_RAW; ++x) mbar_wait(&full[x], 0);
     } else {
       // ---------------------------------------------------------- MMA issuer of lane r
       const int r = warp - 13;
