@@ -17,8 +17,9 @@ namespace {
 constexpr int KP_NS = 3;                                  // K/V ring depth (32 KB per stage)
 constexpr int KP_RAW = 3, RAW_BYTES = 128 * 36;           // blocks of codes and scales on their way, per operand
 constexpr int KP_THREADS = 512;
+constexpr int KP_SORT = 256;                               // most pairs of a slot and a pair of tiles that are sorted by their cost
 constexpr int KP_SMEM = 4 * T128 /*Q: 2 buffers x 2 tiles*/ + KP_NS * 2 * T128 /*K,V ring*/ + 2 * KP_RAW * RAW_BYTES /*codes and scales*/ + 1024 /*alignment*/ + 512 /*barriers*/ +
-                        4096 /*row statistics*/ + 2048 /*row factors*/;
+                        2048 /*row sums*/ + 2048 /*row factors*/ + KP_SORT * 20 /*slots and pairs of tiles by cost*/;
 constexpr uint32_t IDESC_QK = make_idesc(FMT_F16, FMT_F16, 0, 0, 128, 128);
 constexpr uint32_t IDESC_PV = make_idesc(FMT_F16, FMT_F16, 0, 1, 128, 64);     // A (P) K-major from TMEM, B (V) stored [keys, HS]
 constexpr float P_SHIFT = 7.f;                            // P <= 2^(7 + 8)
@@ -42,20 +43,21 @@ __device__ __forceinline__ void unpack8(uint32_t w, uint32_t (&h)[4]) {
 
 // A work item: one (slot, key head) and the query tiles t0, t0 + 1 (tpi 2; or t0 alone).  nb: key blocks that the tile sees, 0 where it has no
 // rows or sees nothing; the second tile sees no fewer than the first unless it has no rows.
+//
+// Items are dealt out by decreasing cost, forwards and backwards in turns.  What a slot's tiles cost is known on the device alone: where there are
+// no more than KP_SORT pairs of a slot and a pair of tiles, every CTA sorts those by the blocks that they see (16 ragged prompts of up to 1000
+// tokens: at most 27 blocks on a CTA, 24.9 on average; 31 by the pairs alone).  Else the last pairs of all slots come first.
 struct KpItem { int s, h, t0, len, cnt, rows[2], nb[2], most; bool valid; };
-struct KpGrid { int n_t, n_pairs, gpw, units, tpi; };
+struct KpGrid { int n_pairs, tpi, sorted; };
+struct KpEntry { int s, pair, len, cnt; };
 __device__ __forceinline__ int kp_token(const Kv4Attn& p, int row) { return p.group == 1 ? row : row / p.group; }
-__device__ __forceinline__ KpItem kp_item(const Kv4Attn& p, const KpGrid& g, int k) {
-  const int c = blockIdx.x, grp = c / g.n_pairs, unit = k * g.gpw + grp;
+__device__ __forceinline__ KpEntry kp_entry(const Kv4Attn& p, int s, int pair) {
+  return KpEntry{s, pair, min(max(p.lens[s], 0), p.d.capacity), p.counts ? min(max(p.counts[s], 0), p.n) : p.n};
+}
+__device__ __forceinline__ KpItem kp_of(const Kv4Attn& p, const KpGrid& g, const KpEntry& e, int h) {
   KpItem it;
-  it.valid = grp < g.gpw && unit < g.units;
-  it.s = it.valid ? unit / p.d.heads : 0; it.h = unit - it.s * p.d.heads;
-  it.t0 = g.tpi * ((c % g.n_pairs + k) % g.n_pairs);
-  it.len = it.cnt = it.most = 0;
-  it.rows[0] = it.rows[1] = it.nb[0] = it.nb[1] = 0;
-  if (!it.valid) return it;
-  it.len = min(max(p.lens[it.s], 0), p.d.capacity);
-  it.cnt = p.counts ? min(max(p.counts[it.s], 0), p.n) : p.n;
+  it.valid = true;
+  it.s = e.s; it.h = h; it.t0 = g.tpi * e.pair; it.len = e.len; it.cnt = e.cnt;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const int first = (it.t0 + t) * TILE;
@@ -64,6 +66,16 @@ __device__ __forceinline__ KpItem kp_item(const Kv4Attn& p, const KpGrid& g, int
   }
   it.most = max(it.nb[0], it.nb[1]);
   return it;
+}
+// item k of this CTA
+__device__ __forceinline__ KpItem kp_item(const Kv4Attn& p, const KpGrid& g, const KpEntry* order, int k) {
+  const long long index = (long long)k * gridDim.x + (k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+  const int entries = p.d.slots * g.n_pairs;              // times heads below 2^31 (host)
+  if (index >= (long long)entries * p.d.heads) { KpItem none; none.valid = false; none.most = 0; return none; }
+  const int entry = (int)index / p.d.heads, h = (int)index - entry * p.d.heads;
+  if (g.sorted) return kp_of(p, g, order[entry], h);
+  const int back = entry / p.d.slots;
+  return kp_of(p, g, kp_entry(p, entry - back * p.d.slots, g.n_pairs - 1 - back), h);
 }
 
 __global__ void __launch_bounds__(KP_THREADS, 1) attention_kv4_prompt_kernel(const Kv4Attn p, const KpGrid grid, const int o_vec) {
@@ -86,7 +98,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) attention_kv4_prompt_kernel(con
   uint64_t* raw_full = fin + 2;                           // [2][RAW] a block's codes and scales are in shared memory
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_full + 2 * KP_RAW);
   float* stats = reinterpret_cast<float*>(bars + 64);     // [lane][item parity][l][128 rows] (m is not needed)
-  float* factor = stats + 1024;                           // [qb][tile][128 rows]: products to log2 units
+  float* factor = stats + 512;                            // [qb][tile][128 rows]: products to log2 units
+  KpEntry* order = reinterpret_cast<KpEntry*>(factor + 512);               // by decreasing cost
+  int* cost = reinterpret_cast<int*>(order + KP_SORT);
 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   if (tid == 0) {
@@ -107,6 +121,23 @@ __global__ void __launch_bounds__(KP_THREADS, 1) attention_kv4_prompt_kernel(con
   bool failed = false;
   pdl_trigger();
   pdl_wait();
+  if (grid.sorted) {
+    const int entries = p.d.slots * grid.n_pairs;         // at most KP_SORT < KP_THREADS
+    KpEntry mine{};
+    if (tid < entries) {
+      const int pair = tid / p.d.slots;
+      mine = kp_entry(p, tid - pair * p.d.slots, pair);
+      const KpItem it = kp_of(p, grid, mine, 0);
+      cost[tid] = it.rows[0] ? it.most + 1 : 0;
+    }
+    __syncthreads();
+    if (tid < entries) {
+      int rank = 0;
+      for (int o = 0; o < entries; ++o) rank += cost[o] > cost[tid] || (cost[o] == cost[tid] && o < tid);
+      order[rank] = mine;
+    }
+    __syncthreads();
+  }
   // Registers: 2 x 128 x 176 + 2 x 128 x 80 = 65536 = the 512 x 128 that the CTA was launched with; each role sets its limit in its own branch.
   if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
@@ -120,11 +151,11 @@ __global__ void __launch_bounds__(KP_THREADS, 1) attention_kv4_prompt_kernel(con
       unsigned char* raw = sRaw + (is_v ? KP_RAW * RAW_BYTES : 0);
       uint64_t* full = raw_full + (is_v ? KP_RAW : 0);
       const int half = lane & 1, key0 = lane >> 1;        // a lane takes half a row, 16 bytes of codes, of the rows key0 + 16 x
-      KpItem it = kp_item(p, grid, 0);
+      KpItem it = kp_item(p, grid, order, 0);
       int k = 0, j = 0, issued = 0;
       uint32_t state = 0;                                 // four bits per stage: page 0 / 1 names no slot, page 1 lies behind the cache
       auto issue = [&]() {
-        while (it.valid && j >= it.most) { j = 0; it = kp_item(p, grid, ++k); }
+        while (it.valid && j >= it.most) { j = 0; it = kp_item(p, grid, order, ++k); }
         if (!it.valid) return;
         const int st = issued % KP_RAW, page0 = 2 * j, pages = p.d.capacity / PAGE;
         const bool two = page0 + 1 < pages;
@@ -197,7 +228,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) attention_kv4_prompt_kernel(con
       const uint64_t k_desc0 = make_smem_desc(smem_u32(sKV), 16, 1024);
       const uint64_t v_desc0 = make_smem_desc(smem_u32(sKV + T128), 8192, 1024);
       for (int k = 0; !failed; ++k) {
-        const KpItem it = kp_item(p, grid, k);
+        const KpItem it = kp_item(p, grid, order, k);
         if (!it.valid) break;
         const int qb = k & 1, tt = r ^ (k & 1), nbt = tt ? it.nb[1] : it.nb[0];
         const uint64_t q_desc = q_desc0 + (uint64_t)(((qb * 2 + tt) * T128) >> 4);
@@ -263,7 +294,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) attention_kv4_prompt_kernel(con
     const float vunit = pow2(p.d.v_exp);
     int cp[2] = {0, 0}, ni[2] = {0, 0};                   // per lane: products / items so far
     auto load_q = [&](int k) {
-      const KpItem it = kp_item(p, grid, k);
+      const KpItem it = kp_item(p, grid, order, k);
       if (!it.valid) return;
       const int qb = k & 1;
       if (k >= 2 && !(mbar_wait(&q_empty[qb], ((k >> 1) + 1) & 1) && mbar_wait(&q_empty[2 + qb], ((k >> 1) + 1) & 1))) { KP_FAIL(); return; }
@@ -310,7 +341,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) attention_kv4_prompt_kernel(con
     };
     load_q(0);
     for (int k = 0; !failed; ++k) {
-      const KpItem it = kp_item(p, grid, k);
+      const KpItem it = kp_item(p, grid, order, k);
       if (!it.valid) break;
       load_q(k + 1);
       if (failed) break;
@@ -372,7 +403,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) attention_kv4_prompt_kernel(con
     const uint32_t tS = tmem + r * 128 + lane_addr, tO = tmem + 256 + r * 64 + lane_addr, tP = tmem + 384 + r * 64 + lane_addr;
     int cs = 0, cp = 0, ni = 0;
     for (int k = 0; !failed; ++k) {
-      const KpItem it = kp_item(p, grid, k);
+      const KpItem it = kp_item(p, grid, order, k);
       if (!it.valid) break;
       const int tt = r ^ (k & 1), nbt = tt ? it.nb[1] : it.nb[0];
       if (nbt == 0) continue;
@@ -397,10 +428,13 @@ __global__ void __launch_bounds__(KP_THREADS, 1) attention_kv4_prompt_kernel(con
         if (lane == 0) mbar_arrive(&s_free[r]);           // the next block's scores may overwrite S now
         ++cs;
         const int lim = see - j * TILE;
-        if (__any_sync(0xffffffffu, lim < TILE)) {        // keys behind the row's token
 #pragma unroll
-          for (int x = 0; x < 128; ++x)
-            if (x >= lim) s[x] = 0xff800000u;
+        for (int c = 0; c < 4; ++c) {                     // keys behind the row's token
+          if (__any_sync(0xffffffffu, lim < 32 * (c + 1))) {
+#pragma unroll
+            for (int x = 32 * c; x < 32 * (c + 1); ++x)
+              if (x >= lim) s[x] = 0xff800000u;
+          }
         }
         float mx4[4];                                     // four independent chains: the row maximum is latency, not work
 #pragma unroll
@@ -479,16 +513,14 @@ int kv4_attention_prompt(const Kv4Attn& p, cudaStream_t st) {
   if (e) return (int)e;
   const long long rows = (long long)p.n * p.group, units = (long long)p.d.slots * p.d.heads;
   KpGrid g{};
-  g.n_t = (int)ceil_div_ll(rows, TILE);
-  g.units = (int)units;
+  const long long n_t = ceil_div_ll(rows, TILE);
   // pairs of tiles share the key blocks; where the chip has an SM for every tile, a tile alone gets an SM's exponential unit to itself
-  g.tpi = g.n_t * units <= sm_count() ? 1 : 2;
-  g.n_pairs = ceil_div(g.n_t, g.tpi);
+  g.tpi = n_t * units <= sm_count() ? 1 : 2;
+  g.n_pairs = (int)ceil_div_ll(n_t, g.tpi);
   const long long items = g.n_pairs * units;
-  int ctas = sm_count();
-  if (items < ctas) ctas = (int)items;
-  if (ctas < g.n_pairs) ctas = g.n_pairs;                 // one (slot, head) needs n_pairs CTAs side by side
-  g.gpw = max(1, (int)min((long long)(ctas / g.n_pairs), units));
+  if (items > 0x7fffffffLL) return LLMB_ERR_BAD_ARG;
+  g.sorted = p.counts != nullptr && (long long)p.d.slots * g.n_pairs <= KP_SORT;
+  const int ctas = items < sm_count() ? (int)items : sm_count();
   const bool o_vec = ((reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.ob * 2) | (uintptr_t)(p.ot * 2) | (uintptr_t)(p.oh * 2)) & 15) == 0;
   return launch_pdl(attention_kv4_prompt_kernel, ctas, KP_THREADS, KP_SMEM, st, p, g, (int)o_vec);
 }
