@@ -7,6 +7,8 @@ generated token, last-position logits → softmax → CDF sampling → tokenizer
 ``:193-278`` (modes: ``.bin`` / ``.safetensors`` / ``--hf <repo>`` / ``--eval <file>``).
 
     python infer_gpt2.py gpt2_124M.bin --prompt-tokens 50256 --tokens 64
+    python infer_gpt2.py gpt2_124M.bin --prompt-tokens 50256 --tokens 512 --kv-cache 4bit     # one row per token instead of the whole window
+    python infer_gpt2.py gpt2_124M.bin --prompt-tokens 464,3280 --tokens 32 --beams 4         # beam search over the 4-bit cache
     python infer_gpt2.py d12 --eval hellaswag_val.bin -b 16
 """
 from __future__ import annotations
@@ -17,7 +19,7 @@ import time
 
 import torch
 
-from llm_mojo_b200.models import GPT2
+from llm_mojo_b200.models import GPT2, CachedDecoder, beam_search
 from llm_mojo_b200 import ops
 from llm_mojo_b200.utils.eval_dataloader import EvalDataLoader, eval_stat_correct
 from llm_mojo_b200.utils.sampler import SamplerRNG, sample_softmax
@@ -59,6 +61,44 @@ def run_infer(model: GPT2, tokenizer: Tokenizer, prompt, gen_tokens: int, seed: 
     return generated
 
 
+def run_infer_cached(model: GPT2, tokenizer: Tokenizer, prompt, gen_tokens: int, seed: int, temperature: float = 1.0,
+                     out=sys.stdout) -> list:
+    """``run_infer`` with the keys and values kept in 4 bits: the prompt is read once, then each token is one row."""
+    cfg = model.config
+    gen_tokens = min(gen_tokens, cfg.max_seq_len - len(prompt))
+    if gen_tokens <= 0:
+        return []
+    dec = CachedDecoder(model, 1, len(prompt) + gen_tokens)
+    rng = SamplerRNG(seed)
+    generated = []
+    t0 = time.perf_counter()
+    logits = dec.prefill([prompt])
+    for t in range(gen_tokens):
+        probs = ops.softmax_rows(logits, cfg.vocab_size, temperature)[0].float().cpu()
+        cdf = torch.cumsum(probs, 0)
+        nxt = int(min(int(torch.searchsorted(cdf, torch.tensor(rng.random_f32()), right=True)), cfg.vocab_size - 1))
+        generated.append(nxt)
+        out.write(tokenizer.decode(nxt) if tokenizer.has_initialized else f"{nxt} ")
+        out.flush()
+        if t + 1 < gen_tokens:
+            logits = dec.step(torch.tensor([nxt], dtype=torch.int32, device=model.device))
+    dt = time.perf_counter() - t0
+    out.write(f"\n---\n{len(generated)} tokens in {dt:.2f} s ({len(generated) / max(dt, 1e-9):.1f} tok/s)\n")
+    return generated
+
+
+def run_beams(model: GPT2, tokenizer: Tokenizer, prompt, gen_tokens: int, beams: int, length_penalty: float = 0.0, out=sys.stdout) -> list:
+    gen_tokens = min(gen_tokens, model.config.max_seq_len - len(prompt) + 1)
+    if gen_tokens <= 0:
+        return []
+    eos = tokenizer.eot_token if tokenizer.has_initialized and tokenizer.eot_token < model.config.vocab_size else -1
+    best = beam_search(model, [prompt], beams, gen_tokens, eos, length_penalty)[0]
+    for tokens, score in best:
+        text = "".join(tokenizer.decode(t) for t in tokens) if tokenizer.has_initialized else " ".join(map(str, tokens))
+        out.write(f"{score:.4f}  {text}\n")
+    return best
+
+
 def run_eval(model: GPT2, path: str, B: int, T: int) -> float:
     loader = EvalDataLoader(path, B, T)
     correct = 0
@@ -83,6 +123,9 @@ def main(argv=None) -> int:
     ap.add_argument("--tokens", type=int, default=64)
     ap.add_argument("--temperature", type=float, default=1.0)
     ap.add_argument("--seed", type=int, default=1337)
+    ap.add_argument("--kv-cache", choices=["none", "4bit"], default="none", help="keep keys and values (in 4 bits) instead of a whole forward pass per token")
+    ap.add_argument("--beams", type=int, default=0, help="beam search with this many beams instead of sampling (over the 4-bit cache)")
+    ap.add_argument("--length-penalty", type=float, default=0.0, help="beams are ranked by log probability / length ** this in the end")
     ap.add_argument("-b", type=int, default=16)
     ap.add_argument("-t", type=int, default=1024)
     ap.add_argument("--device", default="")
@@ -98,7 +141,12 @@ def main(argv=None) -> int:
         return 0
     tok = Tokenizer(args.tokenizer)
     prompt = [int(x) for x in args.prompt_tokens.split(",")] if args.prompt_tokens else [tok.eot_token]
-    run_infer(model, tok, prompt, args.tokens, args.seed, args.temperature)
+    if args.beams > 0:
+        run_beams(model, tok, prompt, args.tokens, args.beams, args.length_penalty)
+    elif args.kv_cache == "4bit":
+        run_infer_cached(model, tok, prompt, args.tokens, args.seed, args.temperature)
+    else:
+        run_infer(model, tok, prompt, args.tokens, args.seed, args.temperature)
     return 0
 
 

@@ -416,33 +416,49 @@ attention_kv4_mma_kernel(const Kv4Attn p, int log_w, int tiles) {
       }
     }
   }
-  if (W > 1) __syncthreads(); else __syncwarp();
-  const float vunit = pow2(p.d.v_exp);
+  // Joining: what each warp's part of a row counts for, then four columns per lane.  For one block per unit that is the result; a cluster's blocks
+  // (a unit each: W is the whole block) leave the sums of their warps in place of warp 0's part.
+  __shared__ float part[MOST_WARPS][ROWS], um[ROWS], ul[ROWS], share[MOST_SPLITS][ROWS];
   constexpr int PITCH = S::WARP_BYTES / 4;             // floats between two warps' parts
-  float* u0 = reinterpret_cast<float*>(sm + (warp & ~(W - 1)) * S::WARP_BYTES);
-  auto store = [&](int r, int c, float sum, float total) {
-    const int token = token_of(r);
-    const long long at = s * p.ob + token * p.ot + (h * p.group + r0 + r - token * p.group) * p.oh + c;
-    reinterpret_cast<T*>(p.out)[at] = from_f<T>(total == 0.f ? 0.f : sum / total * vunit);
-  };
-  __shared__ float um[ROWS], ul[ROWS], share[MOST_SPLITS][ROWS];
-  for (int x = wi * 32 + lane; x < rows * HD; x += W * 32) {
-    const int r = x / HD, c = x % HD;
-    float mx = -INFINITY, sum = 0.f, total = 0.f;
-    for (int w = 0; w < W; ++w) mx = fmaxf(mx, u0[w * PITCH + ROWS * HD + r]);
+  const int w0 = warp & ~(W - 1);
+  float* u0 = reinterpret_cast<float*>(sm + w0 * S::WARP_BYTES);
+  auto together = [&]() { if (W > 1) __syncthreads(); else __syncwarp(); };
+  together();
+  const float vunit = pow2(p.d.v_exp);
+  for (int x = wi * 32 + lane; x < rows * W; x += W * 32) {
+    const int r = x >> log_w, w = x & (W - 1);
+    float mx = -INFINITY, total = 0.f;
+    for (int y = 0; y < W; ++y) mx = fmaxf(mx, u0[y * PITCH + ROWS * HD + r]);
     const float ref = mx == -INFINITY ? 0.f : mx;
+    for (int y = 0; y < W; ++y) total += u0[y * PITCH + ROWS * HD + ROWS + r] * ex2(u0[y * PITCH + ROWS * HD + r] - ref);
+    const float f = ex2(u0[w * PITCH + ROWS * HD + r] - ref);
+    part[w0 + w][r] = p.splits > 1 ? f : total == 0.f ? 0.f : f / total * vunit;
+    if (w == 0 && p.splits > 1) { um[r] = mx; ul[r] = total; }
+  }
+  together();
+  auto store = [&](int r, int c, float4 v) {
+    const int token = token_of(r);
+    T* at = reinterpret_cast<T*>(p.out) + (s * p.ob + token * p.ot + (h * p.group + r0 + r - token * p.group) * p.oh + c);
+    if (!p.o_vec) { at[0] = from_f<T>(v.x); at[1] = from_f<T>(v.y); at[2] = from_f<T>(v.z); at[3] = from_f<T>(v.w); }
+    else if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(at) = v;
+    else {
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+      *reinterpret_cast<uint2*>(at) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    }
+  };
+  for (int x = wi * 32 + lane; x < rows * (HD / 4); x += W * 32) {
+    const int r = x / (HD / 4), c = x % (HD / 4) * 4;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int w = 0; w < W; ++w) {
-      const float f = ex2(u0[w * PITCH + ROWS * HD + r] - ref);
-      sum += u0[w * PITCH + x] * f; total += u0[w * PITCH + ROWS * HD + ROWS + r] * f;
+      const float4 v = *reinterpret_cast<const float4*>(u0 + w * PITCH + r * HD + c);
+      const float f = part[w0 + w][r];
+      sum.x += v.x * f; sum.y += v.y * f; sum.z += v.z * f; sum.w += v.w * f;
     }
-    if (p.splits == 1) store(r, c, sum, total);
-    else {                                             // a unit per cluster: W is the whole block
-      u0[x] = sum;
-      if (c == 0) { um[r] = mx; ul[r] = total; }
-    }
+    if (p.splits == 1) store(r, c, sum);
+    else *reinterpret_cast<float4*>(u0 + r * HD + c) = sum;
   }
   if (p.splits == 1) return;
-  // The blocks of a cluster: each has its part of every row; each finishes a share of the elements from everybody's.
+  // The blocks of a cluster: each finishes a share of the elements from everybody's.
   cg::cluster_group cluster = cg::this_cluster();
   cluster.sync();
   for (int x = threadIdx.x; x < rows * p.splits; x += blockDim.x) {
@@ -451,14 +467,18 @@ attention_kv4_mma_kernel(const Kv4Attn p, int log_w, int tiles) {
     for (int y = 0; y < p.splits; ++y) mx = fmaxf(mx, *cluster.map_shared_rank(&um[r], y));
     const float ref = mx == -INFINITY ? 0.f : mx;
     for (int y = 0; y < p.splits; ++y) total += *cluster.map_shared_rank(&ul[r], y) * ex2(*cluster.map_shared_rank(&um[r], y) - ref);
-    share[k][r] = total == 0.f ? 0.f : ex2(*cluster.map_shared_rank(&um[r], k) - ref) / total;
+    share[k][r] = total == 0.f ? 0.f : ex2(*cluster.map_shared_rank(&um[r], k) - ref) / total * vunit;
   }
   __syncthreads();
-  for (int x = split * blockDim.x + threadIdx.x; x < rows * HD; x += p.splits * blockDim.x) {
-    const int r = x / HD;
-    float sum = 0.f;
-    for (int k = 0; k < p.splits; ++k) sum += cluster.map_shared_rank(u0, k)[x] * share[k][r];
-    store(r, x % HD, sum, 1.f);
+  for (int x = split * blockDim.x + threadIdx.x; x < rows * (HD / 4); x += p.splits * blockDim.x) {
+    const int r = x / (HD / 4), c = x % (HD / 4) * 4;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < p.splits; ++k) {
+      const float4 v = *reinterpret_cast<const float4*>(cluster.map_shared_rank(u0, k) + r * HD + c);
+      const float f = share[k][r];
+      sum.x += v.x * f; sum.y += v.y * f; sum.z += v.z * f; sum.w += v.w * f;
+    }
+    store(r, c, sum);
   }
   cluster.sync();                                      // no block leaves while another reads its shared memory
 }
@@ -532,8 +552,9 @@ struct Kv4AttendArgs {
 LLMB_API int llmb_attention_kv4(const Kv4Desc* d, const Kv4AttendArgs* a, cudaStream_t st) {
   if (a->heads % d->heads) return LLMB_ERR_BAD_ARG;
   Kv4Attn p{*d, a->out, a->q, a->lens, a->counts, a->pages, a->layer, a->n, a->heads / d->heads, 1, a->scale * 1.4426950408889634f,
-            a->qb, a->qt, a->qh, a->ob, a->ot, a->oh, a->status, false};
+            a->qb, a->qt, a->qh, a->ob, a->ot, a->oh, a->status, false, false};
   const int elt = a->dtype == LLMB_BF16 ? 2 : 4;
+  p.o_vec = ((reinterpret_cast<uintptr_t>(a->out) | (uintptr_t)(a->ob * elt) | (uintptr_t)(a->ot * elt) | (uintptr_t)(a->oh * elt)) & (4 * elt - 1)) == 0;
   p.q_vec = ((reinterpret_cast<uintptr_t>(a->q) | (uintptr_t)(a->qb * elt) | (uintptr_t)(a->qt * elt) | (uintptr_t)(a->qh * elt)) & 15) == 0;
   return a->dtype == LLMB_BF16 ? run_type<__nv_bfloat16>(p, st) : run_type<float>(p, st);
 }

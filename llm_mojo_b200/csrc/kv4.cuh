@@ -60,7 +60,7 @@ struct Kv4Attn {
   float scale_log2;
   long long qb, qt, qh, ob, ot, oh;                    // element strides
   int* status;
-  bool q_vec;                                          // rows of q can be read 16 bytes at a time
+  bool q_vec, o_vec;                                   // rows of q can be read 16 bytes at a time, those of out written four values at a time
 };
 
 // Rows of at least KV4_PROMPT_ROWS on the tcgen05 kernel (bf16, heads of 64): attention_kv4_prompt.cu
