@@ -8,7 +8,7 @@ import torch
 
 from . import _count
 from ._lib import lib
-from .kv4 import _call, _ints
+from .kv4 import _call, _ints, _name
 
 BEAM_MAX = 64
 _SELECT = struct.Struct("@8Pq6i")            # BeamSelectArgs of csrc/beam.cu
@@ -28,13 +28,13 @@ def beam_select(scores_out: torch.Tensor, tokens: torch.Tensor, parents: torch.T
     log-sum-exp (a NaN or +inf among them, or nothing but -inf), offers -inf throughout.  Outputs may not share memory with inputs.
 
     The order within a beam is that of its logits, between beams that of the sums in 64 bits, with each log-sum-exp from fp32 exponentials."""
-    shape, dev = scores.shape, scores.device
+    shape, dev = scores.shape, scores.get_device()
     if len(shape) != 2 or scores.dtype is not torch.float32 or not scores.is_contiguous():
         raise ValueError(f"scores must be a contiguous fp32 [B, K], not {scores.dtype} {tuple(shape)}")
     B, K = shape
     rows, dtype = logits.shape, logits.dtype
-    if len(rows) != 2 or rows[0] != B * K or logits.device != dev or (logits.stride(1) != 1 and logits.numel()):
-        raise ValueError(f"logits must be [{B * K}, at least {vocab_size}] on {dev} with dense rows, not {tuple(rows)} on {logits.device}")
+    if len(rows) != 2 or rows[0] != B * K or logits.get_device() != dev or (logits.stride(1) != 1 and logits.numel()):
+        raise ValueError(f"logits must be [{B * K}, at least {vocab_size}] on {_name(dev)} with dense rows, not {tuple(rows)} on {logits.device}")
     if dtype is not torch.bfloat16 and dtype is not torch.float32:
         raise TypeError(f"logits must be bf16 or fp32, not {dtype}")
     if not 1 <= K <= BEAM_MAX:
@@ -47,8 +47,8 @@ def beam_select(scores_out: torch.Tensor, tokens: torch.Tensor, parents: torch.T
         raise ValueError(f"eos {eos} is no token of a vocabulary of {vocab_size}")
     if finished is not None and eos < 0:
         raise ValueError("finished beams go on with eos: it is needed")
-    if scores_out.dtype is not torch.float32 or scores_out.shape != shape or scores_out.device != dev or not scores_out.is_contiguous():
-        raise ValueError(f"scores_out must be a contiguous fp32 {tuple(shape)} on {dev}")
+    if scores_out.dtype is not torch.float32 or scores_out.shape != shape or scores_out.get_device() != dev or not scores_out.is_contiguous():
+        raise ValueError(f"scores_out must be a contiguous fp32 {tuple(shape)} on {_name(dev)}")
     so, si = scores_out.data_ptr(), scores.data_ptr()
     tk, pa = _ints(tokens, "tokens", shape, dev), _ints(parents, "parents", shape, dev)
     if tokens is None or parents is None:
@@ -59,8 +59,8 @@ def beam_select(scores_out: torch.Tensor, tokens: torch.Tensor, parents: torch.T
     for name, t in (("finished", finished), ("finished_out", finished_out)):
         if t is None:
             continue
-        if t.dtype is not torch.bool or t.shape != shape or t.device != dev or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous bool {tuple(shape)} on {dev}")
+        if t.dtype is not torch.bool or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous bool {tuple(shape)} on {_name(dev)}")
         at = t.data_ptr()
         spans.append((at, n))
         fi, fo = (at, fo) if t is finished else (fi, at)
@@ -72,10 +72,10 @@ def beam_select(scores_out: torch.Tensor, tokens: torch.Tensor, parents: torch.T
         if at < end:
             raise ValueError("outputs must not share memory with each other or with inputs")
         end = at + size
-    if scores.is_cuda:
+    if dev >= 0:
         L = lib()
         # one call's own workspace: it lives as long as the work on this stream, and captured graphs do not share it
-        work = torch.empty(n * -(-vocab_size // 4096) * (8 + 8 * K), dtype=torch.uint8, device=dev)
+        work = torch.empty(n * -(-vocab_size // 4096) * (8 + 8 * K), dtype=torch.uint8, device=scores.device)
         _call(L.llmb_beam_select, "beam_select", dev,
               _SELECT.pack(so, tk, pa, fo, logits.data_ptr(), si, fi, work.data_ptr(), logits.stride(0), B, K, vocab_size, eos, 1 if dtype is torch.bfloat16 else 0, 0))
         _count(2)

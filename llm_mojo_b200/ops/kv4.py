@@ -38,6 +38,8 @@ _ATTEND = struct.Struct("@6P6qf5i")          # Kv4AttendArgs of csrc/attention_k
 
 
 def _exponent(unit: float, name: str) -> int:
+    if unit == KV4_UNIT:
+        return -4
     m, e = math.frexp(unit) if isinstance(unit, (int, float)) and math.isfinite(unit) else (0.0, 0)
     if m != 0.5 or not -32 <= e - 1 <= 32:
         raise ValueError(f"{name} must be a power of two between 2^-32 and 2^32, not {unit!r}")
@@ -49,38 +51,46 @@ class KV4Cache:
     slot, some of the layers); heads, tokens and values lie densely, every row 16-byte aligned."""
 
     __slots__ = ("k_codes", "k_scales", "v_codes", "v_scales", "k_unit", "v_unit", "layers", "slots", "kv_heads", "capacity", "head_size",
-                 "device", "_desc")
+                 "device", "index", "_desc")
 
     def __init__(self, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor,
                  k_unit: float = KV4_UNIT, v_unit: float = KV4_UNIT):
-        if k_codes.dim() != 5:
-            raise ValueError(f"codes are [layers, slots, kv_heads, capacity, head_size / 2], not {tuple(k_codes.shape)}")
-        L, S, H, T, half = k_codes.shape
+        codes, scales = k_codes.shape, k_scales.shape
+        if len(codes) != 5:
+            raise ValueError(f"codes are [layers, slots, kv_heads, capacity, head_size / 2], not {tuple(codes)}")
+        L, S, H, T, half = codes
         if 2 * half not in KV4_HEAD_SIZES:
             raise ValueError(f"head size {2 * half}: the cache takes {KV4_HEAD_SIZES}")
         if T % KV4_PAGE or T == 0 or L == 0 or S == 0 or H == 0:
-            raise ValueError(f"capacity {T} must be a multiple of {KV4_PAGE}, and no dimension of {tuple(k_codes.shape)} empty")
+            raise ValueError(f"capacity {T} must be a multiple of {KV4_PAGE}, and no dimension of {tuple(codes)} empty")
         if H > 65535 or S > 65535 or L > 65535:
             raise ValueError(f"at most 65535 layers, slots and heads, not {L}, {S} and {H}")
-        dev = k_codes.device
-        cs, ss = k_codes.stride(), k_scales.stride()
+        dev, at = k_codes.device, k_codes.get_device()
         p = (k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr())
-        codes, scales = (L, S, H, T, half), (L, S, H, T, half // 8)
-        for name, t, shape, st, at in (("k_codes", k_codes, codes, cs, p[0]), ("k_scales", k_scales, scales, ss, p[1]),
-                                       ("v_codes", v_codes, codes, cs, p[2]), ("v_scales", v_scales, scales, ss, p[3])):
-            if t.dtype is not torch.uint8 or t.shape != shape or t.device != dev:
-                raise ValueError(f"{name} must be uint8 {shape} on {dev}, not {t.dtype} {tuple(t.shape)} on {t.device}")
-            if t.stride() != st:
-                raise ValueError(f"{name}: keys and values must have the same strides, not {t.stride()} and {st}")
-            c = shape[4]
-            if st[4] != 1 or st[3] != c or (H > 1 and st[2] != T * c) or (at | (st[1] if S > 1 else 0) | (st[0] if L > 1 else 0)) % 16:
-                raise ValueError(f"{name}: heads, tokens and values must lie densely, slots and layers 16-byte aligned (strides {st})")
-            row = H * T * c
-            if (S > 1 and st[1] < row) or (L > 1 and st[0] < row) or (L > 1 and S > 1 and (S - 1) * st[1] + row > st[0] and (L - 1) * st[0] + row > st[1]):
-                raise ValueError(f"{name}: slots and layers must not overlap (strides {st})")
+        u8 = torch.uint8
+        if (scales != (L, S, H, T, half // 8) or v_codes.shape != codes or v_scales.shape != scales or k_scales.get_device() != at
+                or v_codes.get_device() != at or v_scales.get_device() != at or k_codes.dtype is not u8 or k_scales.dtype is not u8
+                or v_codes.dtype is not u8 or v_scales.dtype is not u8):
+            for name, t, shape in (("k_codes", k_codes, tuple(codes)), ("k_scales", k_scales, (L, S, H, T, half // 8)),
+                                   ("v_codes", v_codes, tuple(codes)), ("v_scales", v_scales, (L, S, H, T, half // 8))):
+                if t.dtype != u8 or t.shape != shape or t.device != dev:
+                    raise ValueError(f"{name} must be uint8 {shape} on {dev}, not {t.dtype} {tuple(t.shape)} on {t.device}")
+        cs, ss = k_codes.stride(), k_scales.stride()
+        if (p[0] | p[1] | p[2] | p[3]) % 16 or not (k_codes.is_contiguous() and k_scales.is_contiguous() and v_codes.is_contiguous()
+                                                    and v_scales.is_contiguous()):
+            for name, t, st, ptr in (("k_codes", k_codes, cs, p[0]), ("k_scales", k_scales, ss, p[1]), ("v_codes", v_codes, cs, p[2]),
+                                     ("v_scales", v_scales, ss, p[3])):
+                if t.stride() != st:
+                    raise ValueError(f"{name}: keys and values must have the same strides, not {t.stride()} and {st}")
+                c = t.shape[4]
+                if st[4] != 1 or st[3] != c or (H > 1 and st[2] != T * c) or (ptr | (st[1] if S > 1 else 0) | (st[0] if L > 1 else 0)) % 16:
+                    raise ValueError(f"{name}: heads, tokens and values must lie densely, slots and layers 16-byte aligned (strides {st})")
+                row = H * T * c
+                if (S > 1 and st[1] < row) or (L > 1 and st[0] < row) or (L > 1 and S > 1 and (S - 1) * st[1] + row > st[0] and (L - 1) * st[0] + row > st[1]):
+                    raise ValueError(f"{name}: slots and layers must not overlap (strides {st})")
         self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
         self.k_unit, self.v_unit = k_unit, v_unit
-        self.layers, self.slots, self.kv_heads, self.capacity, self.head_size, self.device = L, S, H, T, 2 * half, dev
+        self.layers, self.slots, self.kv_heads, self.capacity, self.head_size, self.device, self.index = L, S, H, T, 2 * half, dev, at
         self._desc = _DESC.pack(*p, cs[0], cs[1], ss[0], ss[1], L, S, H, T, 2 * half, _exponent(k_unit, "k_unit"), _exponent(v_unit, "v_unit"), 0)
 
     @classmethod
@@ -110,25 +120,31 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_get
     lambda index: torch.cuda.current_stream(index).cuda_stream
 
 
-def _call(fn, name: str, device: torch.device, *args) -> None:
+_current = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
+def _call(fn, name: str, index: int, *args) -> None:
     """Launches go to the current stream of the tensors' device, whichever device is current."""
-    index = device.index
-    if index == torch.cuda.current_device():
+    if index == _current():
         rc = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             rc = fn(*args, _raw_stream(index))
     if rc:
         check(rc, name)
 
 
-def _ints(t: Optional[torch.Tensor], name: str, shape: tuple, device) -> int:
+def _ints(t: Optional[torch.Tensor], name: str, shape: tuple, index: int) -> int:
     """The address of an optional tensor of integers."""
     if t is None:
         return 0
-    if t.dtype is not torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 {shape} on {device}, not {t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.dtype is not torch.int32 or t.shape != shape or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 {tuple(shape)} on {_name(index)}, not {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
+
+
+def _name(index: int) -> str:
+    return f"cuda:{index}" if index >= 0 else "cpu"
 
 
 def _layer(cache: KV4Cache, layer: int) -> None:
@@ -136,10 +152,10 @@ def _layer(cache: KV4Cache, layer: int) -> None:
         raise ValueError(f"layer {layer!r} of a cache of {cache.layers} layers")
 
 
-def _rows(t: torch.Tensor, name: str, shape: tuple, dtype, device) -> tuple:
+def _rows(t: torch.Tensor, name: str, shape: tuple, dtype, index: int) -> tuple:
     """The strides of a tensor of rows."""
-    if t.dtype is not dtype or t.shape != shape or t.device != device:
-        raise ValueError(f"{name} must be {dtype} {tuple(shape)} on {device}, not {t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != index:
+        raise ValueError(f"{name} must be {dtype} {tuple(shape)} on {_name(index)}, not {t.dtype} {tuple(t.shape)} on {t.device}")
     st = t.stride()
     if st[-1] != 1 and t.numel():
         raise ValueError(f"{name}: the values of a head must lie densely (strides {st})")
@@ -188,7 +204,7 @@ def kv4_append(cache: KV4Cache, layer: int, k: torch.Tensor, v: torch.Tensor, st
     if len(shape) != 4 or shape[0] != cache.slots or shape[2] != cache.kv_heads or shape[3] != cache.head_size:
         raise ValueError(f"k must be [{cache.slots}, n, {cache.kv_heads}, {cache.head_size}], not {tuple(shape)}")
     S, n, H, hd = shape
-    dtype, dev = k.dtype, cache.device
+    dtype, dev = k.dtype, cache.index
     if dtype is not torch.bfloat16 and dtype is not torch.float32:
         raise TypeError(f"k and v must be bf16 or fp32, not {dtype}")
     _layer(cache, layer)
@@ -196,7 +212,7 @@ def kv4_append(cache: KV4Cache, layer: int, k: torch.Tensor, v: torch.Tensor, st
     at, cnt = _ints(start, "start", (S,), dev), _ints(counts, "counts", (S,), dev)
     if n == 0:
         return
-    if k.is_cuda:
+    if dev >= 0:
         _call(lib().llmb_kv4_append, "kv4_append", dev, cache._desc,
               _APPEND.pack(k.data_ptr(), v.data_ptr(), at, cnt, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], layer, n, 1 if dtype is torch.bfloat16 else 0, 0))
         _count()
@@ -220,7 +236,7 @@ def kv4_values(k_out: torch.Tensor, v_out: torch.Tensor, cache: KV4Cache, layer:
     """Reads back what the cache holds: ``k_out``, ``v_out`` [slots, n, kv_heads, head_size] (bf16, in which every value is exact, or fp32) of
     the positions ``start[s] + i`` of one layer, or [layers, slots, ...] of all layers (``layer`` None).  Positions outside the cache read as
     zeros, pages whose entry in ``pages`` names no slot as NaN."""
-    dtype, dev, shape = k_out.dtype, cache.device, k_out.shape
+    dtype, dev, shape = k_out.dtype, cache.index, k_out.shape
     lead = (cache.slots,) if layer is not None else (cache.layers, cache.slots)
     if len(shape) != len(lead) + 3 or shape[:-3] != lead or shape[-2] != cache.kv_heads or shape[-1] != cache.head_size:
         raise ValueError(f"k_out must be {[*lead, 'n', cache.kv_heads, cache.head_size]}, not {tuple(shape)}")
@@ -237,7 +253,7 @@ def kv4_values(k_out: torch.Tensor, v_out: torch.Tensor, cache: KV4Cache, layer:
     at, pg = _ints(start, "start", (cache.slots,), dev), _ints(pages, "pages", (cache.slots, cache.capacity // KV4_PAGE), dev)
     if n == 0:
         return
-    if k_out.is_cuda:
+    if dev >= 0:
         _call(lib().llmb_kv4_values, "kv4_values", dev, cache._desc,
               _VALUES.pack(k_out.data_ptr(), v_out.data_ptr(), at, pg, ks[0] if layer is None else 0, ks[-4], ks[-3], ks[-2], vs[-4], vs[-3], vs[-2],
                            -1 if layer is None else layer, n, 1 if dtype is torch.bfloat16 else 0, 0))
@@ -270,7 +286,7 @@ def attention_kv4(out: torch.Tensor, q: torch.Tensor, cache: KV4Cache, layer: in
     ``out`` may be ``q`` itself.  A page whose entry in ``pages`` names no slot gives NaN to every row that sees it.
 
     Scores, statistics and sums are in fp32.  lens above the capacity count as the capacity."""
-    shape, dtype, dev = q.shape, q.dtype, cache.device
+    shape, dtype, dev = q.shape, q.dtype, cache.index
     if len(shape) != 4 or shape[0] != cache.slots or shape[3] != cache.head_size or shape[2] % cache.kv_heads or shape[2] == 0:
         raise ValueError(f"q must be [{cache.slots}, n, a multiple of {cache.kv_heads}, {cache.head_size}], not {tuple(shape)}")
     if dtype is not torch.bfloat16 and dtype is not torch.float32:
@@ -288,9 +304,9 @@ def attention_kv4(out: torch.Tensor, q: torch.Tensor, cache: KV4Cache, layer: in
         raise ValueError(f"{n} rows of {heads} heads are too many")
     if n == 0:
         return
-    if q.is_cuda:
+    if dev >= 0:
         _call(lib().llmb_attention_kv4, "attention_kv4", dev, cache._desc,
-              _ATTEND.pack(out.data_ptr(), q.data_ptr(), ln, cnt, pg, status_word(dev).data_ptr(), qs[0], qs[1], qs[2], os_[0], os_[1], os_[2], scale, layer, n,
+              _ATTEND.pack(out.data_ptr(), q.data_ptr(), ln, cnt, pg, status_word(cache.device).data_ptr(), qs[0], qs[1], qs[2], os_[0], os_[1], os_[2], scale, layer, n,
                            heads, 1 if dtype is torch.bfloat16 else 0, 0))
         _count()
         return
@@ -330,12 +346,12 @@ def kv4_reorder(cache: KV4Cache, pages: torch.Tensor, lens: torch.Tensor, parent
     B, K = parents.shape
     if K > 64:
         raise ValueError(f"at most 64 beams, not {K}")
-    dev = cache.device
+    dev = cache.index
     if pages is None or lens is None:
         raise ValueError("kv4_reorder permutes pages and lens: both are needed")
     par, ln = _ints(parents, "parents", (B, K), dev), _ints(lens, "lens", (cache.slots,), dev)
     pg = _ints(pages, "pages", (cache.slots, cache.capacity // KV4_PAGE), dev)
-    if lens.is_cuda:
+    if dev >= 0:
         _call(lib().llmb_kv4_reorder, "kv4_reorder", dev, cache._desc, pg, ln, par, K)
         _count(2)
         return
