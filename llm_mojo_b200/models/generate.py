@@ -53,7 +53,7 @@ class CachedDecoder:
         before = lens.clone()
         lens += n if counts is None else counts
         pos = (before.long().view(S, 1) + torch.arange(n, device=m.device)).clamp_(max=cfg.max_seq_len - 1)
-        x = (p["wte"][tokens.long().view(-1)] + p["wpe"][pos.view(-1)])
+        x = p["wte"][tokens.long().view(-1).clamp(0, cfg.vocab_size - 1)] + p["wpe"][pos.view(-1)]        # an index from outside addresses nothing
         ln, mean, rstd, qkv, att, pre, act = e(rows, C), e(rows, dtype=torch.float32), e(rows, dtype=torch.float32), e(rows, 3 * C), e(rows, C), e(rows, 4 * C), e(rows, 4 * C)
         heads = qkv.view(S, n, 3, NH, hd)
         q, k, v = heads[:, :, 0], heads[:, :, 1], heads[:, :, 2]
@@ -109,7 +109,7 @@ class CachedDecoder:
     @torch.no_grad()
     def step(self, tokens: torch.Tensor) -> torch.Tensor:
         """Appends ``tokens`` (int32 [slots] or [slots, 1] on the model's device), one to every text; returns the logits behind them.  The
-        result is overwritten by the next step."""
+        result is overwritten by the next step.  Tokens outside the vocabulary, which only the device knows, count as the nearest in it."""
         if tokens.numel() != self.slots:
             raise ValueError(f"one token for each of {self.slots} texts, not {tuple(tokens.shape)}")
         self._grow(1)

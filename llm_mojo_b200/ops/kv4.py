@@ -63,8 +63,8 @@ class KV4Cache:
             raise ValueError(f"head size {2 * half}: the cache takes {KV4_HEAD_SIZES}")
         if T % KV4_PAGE or T == 0 or L == 0 or S == 0 or H == 0:
             raise ValueError(f"capacity {T} must be a multiple of {KV4_PAGE}, and no dimension of {tuple(codes)} empty")
-        if H > 65535 or S > 65535 or L > 65535:
-            raise ValueError(f"at most 65535 layers, slots and heads, not {L}, {S} and {H}")
+        if H > 65535 or S > 65535 or L > 65535 or T > 2 ** 30:
+            raise ValueError(f"at most 65535 layers, slots and heads and 2^30 tokens, not {L}, {S}, {H} and {T}")
         dev, at = k_codes.device, k_codes.get_device()
         p = (k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr())
         u8 = torch.uint8
@@ -248,6 +248,8 @@ def kv4_values(k_out: torch.Tensor, v_out: torch.Tensor, cache: KV4Cache, layer:
     ks, vs = _rows(k_out, "k_out", shape, dtype, dev), _rows(v_out, "v_out", shape, dtype, dev)
     _spread(k_out, "k_out")
     _spread(v_out, "v_out")
+    if n and k_out.data_ptr() == v_out.data_ptr():
+        raise ValueError("k_out and v_out are two outputs: they must not be the same memory")
     if layer is None and n and ks != vs:
         raise ValueError(f"k_out and v_out must have the same strides, not {ks} and {vs}")
     at, pg = _ints(start, "start", (cache.slots,), dev), _ints(pages, "pages", (cache.slots, cache.capacity // KV4_PAGE), dev)

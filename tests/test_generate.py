@@ -138,6 +138,13 @@ def test_refusals():
         beam_search(m, [[1] * 90], 2, 8)
 
 
+def test_a_token_from_outside_counts_as_the_nearest():
+    m = make()
+    a, b = CachedDecoder(m, 2), CachedDecoder(m, 2)
+    a.prefill([[1, 2], [3]]), b.prefill([[1, 2], [3]])
+    assert torch.equal(a.step(torch.tensor([-5, 10 ** 6], dtype=torch.int32)), b.step(torch.tensor([0, 209], dtype=torch.int32)))
+
+
 def test_command_line(tmp_path):
     from llm_mojo_b200.utils import checkpointing as ckpt
     m = make()

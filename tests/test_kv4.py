@@ -106,6 +106,8 @@ def test_cache_refusals():
         ops.KV4Cache(*(x[:, :1].expand(1, 2, *x.shape[2:]) for x in t))
     with pytest.raises(ValueError, match="layers"):
         ops.KV4Cache(*(x[0] for x in t))
+    with pytest.raises(ValueError, match="2\\^30"):
+        ops.KV4Cache(*(torch.empty(1, 1, 1, 2 ** 31, c, dtype=torch.uint8, device="meta") for c in (32, 4, 32, 4)))
     assert c.select(slice(0, None, 2)).slots == 1
     assert _cache(layers=2, slots=6).select(slice(0, None, 4)).slots == 2
     with pytest.raises(ValueError, match="overlap"):
@@ -134,6 +136,8 @@ def test_append_and_values_refusals():
         ops.kv4_values(torch.zeros(2, 1, 2, 64).expand(2, 3, 2, 64), x, c, 0, z)
     with pytest.raises(ValueError, match="k_out"):
         ops.kv4_values(x, x.clone(), c, None, z)
+    with pytest.raises(ValueError, match="same memory"):
+        ops.kv4_values(x, x, c, 0, z)
     with pytest.raises(ValueError, match="pages"):
         ops.kv4_values(x, x.clone(), c, 0, z, pages=torch.zeros(2, 2, dtype=torch.int32))
     ops.kv4_append(c, 0, x[:, :0], x[:, :0], z)              # nothing to do is no error
