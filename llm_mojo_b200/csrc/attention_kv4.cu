@@ -21,7 +21,7 @@ namespace {
 //      first column, which gives the even columns of o, and (0, p) in its second, the odd ones; with more rows two byte permutations
 //      of every four values make pairs of keys.
 // code x scale is exact in f16.  q is brought into f16's range by a power of two per row (exact for bf16; an fp32 row takes two columns, its
-// upper and its lower 11 bits), P is scaled by 2^15 (the rest of f16's range) and, for fp32, split alike.  P^T comes out of the accumulators of
+// upper and its lower 11 bits), P is scaled by a power of two into the rest of f16's range and, for fp32, split alike.  P^T comes out of the accumulators of
 // S^T as the second product's other operand by a transposition within the warp (movmatrix).
 //
 // Each warp has a ring of its own of key tiles, filled by untiled bulk copies (a tile is contiguous in each of the four tensors), and
@@ -58,7 +58,7 @@ __device__ __forceinline__ uint32_t high2(uint32_t a) { uint32_t d; asm("{\n\t.r
 __device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) { uint32_t d; asm("min.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b)); return d; }
 __device__ __forceinline__ uint32_t f16x2(float lo, float hi) { uint32_t d; asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo)); return d; }
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-constexpr float P_SHIFT = 15.f;                        // P <= 2^15
+constexpr float P_TOP = 15.f, LAG = 8.f;               // P <= 2^15; with one tile of columns the maximum may lag by 2^8
 
 template <typename T, int HD, int NT, bool NARROW>
 __global__ void __launch_bounds__(MOST_WARPS * 32, MmaShape<T, HD, NT, NARROW>::WARPS_SM / MOST_WARPS)
@@ -92,20 +92,27 @@ attention_kv4_mma_kernel(const Kv4Attn p, int log_w, int tiles) {
   const uint32_t dst = tc05::smem_u32(ring) + (lane & 1 ? S::CODE_BYTES : 0) + (lane & 2 ? S::CODE_BYTES + S::SCALE_BYTES : 0);
   src += p.layer * (lane & 1 ? p.d.scale_layer : p.d.code_layer) + (long long)h * cap_tiles * piece;
   int slot_of = s, bad = 0;                            // bad: bit per stage, its page names no slot
+  const unsigned char* next_src = src + s * src_slot + (long long)first * piece;          // of the warp's next tile, in its own slot
+  const long long hop = (long long)step * piece;
   auto issue = [&](int i) {
-    if (p.pages && i % 32 == 0) {
-      const int t = first + (i + lane) * step;
-      slot_of = t < cap_tiles ? p.pages[(long long)s * (p.d.capacity / PAGE) + t * TK / PAGE] : s;
-    }
-    int slot = __shfl_sync(0xffffffffu, slot_of, i % 32);
     const int st = i % NSTG;
-    bad &= ~(1 << st);
-    if (slot < 0 || slot >= p.d.slots) { bad |= 1 << st; slot = s; }
+    const unsigned char* from = next_src;
+    next_src += hop;
+    if (p.pages) {
+      if (i % 32 == 0) {
+        const int t = first + (i + lane) * step;
+        slot_of = t < cap_tiles ? p.pages[(long long)s * (p.d.capacity / PAGE) + t * TK / PAGE] : s;
+      }
+      int slot = __shfl_sync(0xffffffffu, slot_of, i % 32);
+      bad &= ~(1 << st);
+      if (slot < 0 || slot >= p.d.slots) { bad |= 1 << st; slot = s; }
+      from += (slot - s) * src_slot;
+    }
     if (lane == 0) tc05::mbar_expect_tx(&bar[st], S::STAGE);
     __syncwarp();
     if (lane < 4)
       asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                   ::"r"(dst + st * S::STAGE), "l"(src + slot * src_slot + (long long)(first + i * step) * piece), "r"(piece), "r"(tc05::smem_u32(&bar[st])) : "memory");
+                   ::"r"(dst + st * S::STAGE), "l"(from), "r"(piece), "r"(tc05::smem_u32(&bar[st])) : "memory");
   };
   const bool early = here && first < cap_tiles;
   if (early) issue(0);
@@ -177,11 +184,13 @@ attention_kv4_mma_kernel(const Kv4Attn p, int log_w, int tiles) {
     for (int y = 0; y < CPL; ++y) cf[t][y] = __shfl_sync(0xffffffffu, c, 4 * (2 * j + y));
   }
 
-  float o[NWV][NO][NT][4], m[NT][CPL], l[NT][CPL];     // m: of the products, not yet times c
+  // m: the reference maximum of the products, not yet times c; ref: what is added to the products times c; lag: how far they may pass m
+  constexpr float SHIFT = NT == 1 ? P_TOP - LAG : P_TOP;
+  float o[NWV][NO][NT][4], m[NT][CPL], l[NT][CPL], ref[NT][CPL], lag[NT][CPL];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
 #pragma unroll
-    for (int c = 0; c < CPL; ++c) { m[t][c] = -INFINITY; l[t][c] = 0.f; }
+    for (int c = 0; c < CPL; ++c) { m[t][c] = -INFINITY; l[t][c] = 0.f; ref[t][c] = SHIFT; lag[t][c] = NT == 1 ? LAG / cf[t][c] : 0.f; }
 #pragma unroll
     for (int i = 0; i < NWV; ++i)
 #pragma unroll
@@ -276,25 +285,29 @@ attention_kv4_mma_kernel(const Kv4Attn p, int log_w, int tiles) {
       uint32_t pf[G16][NT][NARROW ? 4 : 2];            // NARROW: the two operands of the lower eight keys, then of the upper
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        bool moved = false;
-        float mx[CPL], al[CPL], ref[CPL];
+        float mx[CPL];
 #pragma unroll
         for (int c = 0; c < CPL; ++c) {
           mx[c] = fmaxf(sc[0][t][c], sc[0][t][2 + c]);
 #pragma unroll
           for (int a = 1; a < G16; ++a) mx[c] = fmaxf(mx[c], fmaxf(sc[a][t][c], sc[a][t][2 + c]));
-          mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 4));
-          mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 8));
-          mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 16));
-          const float mn = fmaxf(m[t][c], mx[c]), safe = mn == -INFINITY ? 0.f : mn;
-          al[c] = ex2((m[t][c] - safe) * cf[t][c]);
-          moved |= mn != m[t][c];
-          ref[c] = P_SHIFT - safe * cf[t][c];
-          m[t][c] = mn;
         }
-        if (__any_sync(0xffffffffu, moved)) {
+        // A lane's own maximum says whether the reference has to move: mostly it has not, and the exchange and the rescaling are left out.
+        bool move = mx[0] > m[t][0] + lag[t][0];
+        if (CPL == 2) move |= mx[CPL - 1] > m[t][CPL - 1] + lag[t][CPL - 1];
+        if (__any_sync(0xffffffffu, move)) {
+          float al[CPL];
 #pragma unroll
-          for (int c = 0; c < CPL; ++c) l[t][c] *= al[c];
+          for (int c = 0; c < CPL; ++c) {
+            mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 4));
+            mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 8));
+            mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 16));
+            const float mn = fmaxf(m[t][c], mx[c]), safe = mn == -INFINITY ? 0.f : mn;
+            al[c] = ex2((m[t][c] - safe) * cf[t][c]);
+            ref[t][c] = SHIFT - safe * cf[t][c];
+            m[t][c] = mn;
+            l[t][c] *= al[c];
+          }
 #pragma unroll
           for (int x = 0; x < NWV; ++x)
 #pragma unroll
@@ -307,13 +320,13 @@ attention_kv4_mma_kernel(const Kv4Attn p, int log_w, int tiles) {
           const float (&x)[4] = sc[a][t];
           uint32_t lo, hi;
           if (CPL == 2) {
-            const float2 c2 = make_float2(cf[t][0], cf[t][CPL - 1]), r2 = make_float2(ref[0], ref[CPL - 1]);
+            const float2 c2 = make_float2(cf[t][0], cf[t][CPL - 1]), r2 = make_float2(ref[t][0], ref[t][CPL - 1]);
             const float2 u = __ffma2_rn(make_float2(x[0], x[1]), c2, r2), v = __ffma2_rn(make_float2(x[2], x[3]), c2, r2);
             const float p0 = ex2(u.x), p1 = ex2(u.y), p2 = ex2(v.x), p3 = ex2(v.y);
             l[t][0] += p0 + p2; l[t][CPL - 1] += p1 + p3;
             lo = f16x2(p0, p1); hi = f16x2(p2, p3);
           } else {
-            const float p0 = ex2(fmaf(x[0], cf[t][0], ref[0])), p2 = ex2(fmaf(x[2], cf[t][0], ref[0]));
+            const float p0 = ex2(fmaf(x[0], cf[t][0], ref[t][0])), p2 = ex2(fmaf(x[2], cf[t][0], ref[t][0]));
             l[t][0] += p0 + p2;
             if (PARTS == 1) { lo = f16x2(p0, p0); hi = f16x2(p2, p2); }
             else {
