@@ -239,23 +239,22 @@ __global__ void __launch_bounds__(THREADS) beam_merge_kernel(float* __restrict__
 }
 }  // namespace
 
-// The arguments of a call as the Python side (ops/beam.py) packs them.  work: B K (8 + 8 K) bytes for each 4096 columns.
+// The arguments of a call as the Python side (ops/beam.py) packs them; the workspace is B K (8 + 8 K) bytes for each 4096 columns.
 struct BeamSelectArgs {
   float* scores_out; int *tokens, *parents; bool* finished_out;          // finished_out: optional
   const void* logits; const float* scores; const bool* finished;         // finished: optional
-  void* work;
   long long ld;
   int B, K, V, eos, dtype, pad;
 };
 
-LLMB_API int llmb_beam_select(const BeamSelectArgs* a, cudaStream_t st) {
+LLMB_API int llmb_beam_select(const BeamSelectArgs* a, void* work, cudaStream_t st) {
   const int K = a->K, V = a->V, rows = a->B * K;
   // Chunks of 4096 columns; of 8192, for which a block takes two thirds of the instructions of two, where there are blocks enough (48 x 8 fp32: 34 us in
   // chunks of 4096, 28.6 in chunks of 8192; 38 with the registers that leave two blocks on an SM instead of four).
   const bool wide = (long long)rows * ceil_div(V, 4096) >= 2LL * sm_count() * 8;
   const int chunks = ceil_div(V, wide ? 8192 : 4096);
   if (K < 1 || K > BEAM_MAX || rows > 65535 || (long long)K * chunks * 16 > 46 * 1024) return LLMB_ERR_BAD_ARG;
-  float2* stats = (float2*)a->work;
+  float2* stats = (float2*)work;
   unsigned long long* lists = (unsigned long long*)(stats + (long long)rows * chunks);
   const dim3 grid(chunks, rows);
   auto chunk = [&](auto kernel, auto* logits) { return launch_pdl(kernel, grid, THREADS, 0, st, stats, lists, logits, a->finished, K, V, a->ld, chunks); };

@@ -348,7 +348,11 @@ LLMB_API int llmb_kv4_values(const Kv4Desc* d, const Kv4ValuesArgs* a, cudaStrea
   KV4_HEADS(d->head_size, (values<float, HD>(*d, a->layer, a->k, a->v, a->start, a->pages, a->n, a->out_layer, sk, sv, st)))
 }
 
-LLMB_API int llmb_kv4_reorder(const Kv4Desc* d, int* pages, int* lens, const int* parents, int K, cudaStream_t st) {
+struct Kv4ReorderArgs { int *pages, *lens; const int* parents; int K, pad; };
+
+LLMB_API int llmb_kv4_reorder(const Kv4Desc* d, const Kv4ReorderArgs* a, cudaStream_t st) {
+  int *pages = a->pages, *lens = a->lens, K = a->K;
+  const int* parents = a->parents;
   const int items = K > 0 ? d->slots / K : 0;
   if (K < 1 || K > 64) return LLMB_ERR_BAD_ARG;
   const int threads = K <= 16 ? 128 : K <= 32 ? 64 : 32;        // at most 32 KB of pieces

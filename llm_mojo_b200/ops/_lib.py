@@ -87,9 +87,9 @@ _SIGS = {
     "llmb_attention_bwd_fused_acc_floats": [c_int, c_int, c_int],
     "llmb_kv4_append": [c_p, c_p, c_p],
     "llmb_kv4_values": [c_p, c_p, c_p],
-    "llmb_kv4_reorder": [c_p, c_p, c_p, c_p, c_int, c_p],
+    "llmb_kv4_reorder": [c_p, c_p, c_p],
     "llmb_attention_kv4": [c_p, c_p, c_p],
-    "llmb_beam_select": [c_p, c_p],
+    "llmb_beam_select": [c_p, c_p, c_p],
     "llmb_loss_accumulate": [c_p, c_p, c_int, c_f, c_p],
     "llmb_gpt2_step_bytes": [],
     "llmb_gpt2_lowp_scratch_bytes": [c_p],

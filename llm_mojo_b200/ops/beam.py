@@ -11,7 +11,7 @@ from ._lib import lib
 from .kv4 import _call, _ints, _name
 
 BEAM_MAX = 64
-_SELECT = struct.Struct("@8Pq6i")            # BeamSelectArgs of csrc/beam.cu
+_SELECT = struct.Struct("@7Pq6i")            # BeamSelectArgs of csrc/beam.cu
 
 
 def beam_select(scores_out: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, logits: torch.Tensor, scores: torch.Tensor,
@@ -77,7 +77,7 @@ def beam_select(scores_out: torch.Tensor, tokens: torch.Tensor, parents: torch.T
         # one call's own workspace: it lives as long as the work on this stream, and captured graphs do not share it
         work = torch.empty(n * -(-vocab_size // 4096) * (8 + 8 * K), dtype=torch.uint8, device=scores.device)
         _call(L.llmb_beam_select, "beam_select", dev,
-              _SELECT.pack(so, tk, pa, fo, logits.data_ptr(), si, fi, work.data_ptr(), logits.stride(0), B, K, vocab_size, eos, 1 if dtype is torch.bfloat16 else 0, 0))
+              _SELECT.pack(so, tk, pa, fo, logits.data_ptr(), si, fi, logits.stride(0), B, K, vocab_size, eos, 1 if dtype is torch.bfloat16 else 0, 0), work.data_ptr())
         _count(2)
         return
     x = logits[:, :vocab_size].double().view(B, K, vocab_size)

@@ -34,6 +34,7 @@ _LEVELS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 _DESC = struct.Struct("@4P4q8i")             # Kv4Desc of csrc/kv4.cuh
 _APPEND = struct.Struct("@4P6q4i")           # Kv4AppendArgs of csrc/kv4.cu
 _VALUES = struct.Struct("@4P7q4i")           # Kv4ValuesArgs
+_REORDER = struct.Struct("@3P2i")            # Kv4ReorderArgs
 _ATTEND = struct.Struct("@6P6qf5i")          # Kv4AttendArgs of csrc/attention_kv4.cu
 
 
@@ -123,15 +124,23 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_get
 _current = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 
 
-def _call(fn, name: str, index: int, *args) -> None:
+def _call(fn, name: str, index: int, first, second) -> None:
     """Launches go to the current stream of the tensors' device, whichever device is current."""
     if index == _current():
-        rc = fn(*args, _raw_stream(index))
+        rc = fn(first, second, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, _raw_stream(index))
+            rc = fn(first, second, _raw_stream(index))
     if rc:
         check(rc, name)
+
+
+_STATUS_AT = {}
+
+
+def _status_at(device: torch.device, index: int) -> int:
+    at = _STATUS_AT[index] = status_word(device).data_ptr()      # the word lives as long as the process
+    return at
 
 
 def _ints(t: Optional[torch.Tensor], name: str, shape: tuple, index: int) -> int:
@@ -294,13 +303,16 @@ def attention_kv4(out: torch.Tensor, q: torch.Tensor, cache: KV4Cache, layer: in
     if dtype is not torch.bfloat16 and dtype is not torch.float32:
         raise TypeError(f"q must be bf16 or fp32, not {dtype}")
     S, n, heads, hd = shape
-    _layer(cache, layer)
+    if not isinstance(layer, int) or not 0 <= layer < cache.layers:
+        _layer(cache, layer)
     qs, os_ = _rows(q, "q", shape, dtype, dev), _rows(out, "out", shape, dtype, dev)
-    _spread(out, "out")
+    if not out.is_contiguous():
+        _spread(out, "out")
     ln, cnt = _ints(lens, "lens", (S,), dev), _ints(counts, "counts", (S,), dev)
     pg = _ints(pages, "pages", (S, cache.capacity // KV4_PAGE), dev)
-    scale = hd ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
+    if scale is None:
+        scale = hd ** -0.5
+    elif not math.isfinite(scale):
         raise ValueError(f"scale must be finite, not {scale}")
     if n * heads > 2 ** 30:
         raise ValueError(f"{n} rows of {heads} heads are too many")
@@ -308,7 +320,7 @@ def attention_kv4(out: torch.Tensor, q: torch.Tensor, cache: KV4Cache, layer: in
         return
     if dev >= 0:
         _call(lib().llmb_attention_kv4, "attention_kv4", dev, cache._desc,
-              _ATTEND.pack(out.data_ptr(), q.data_ptr(), ln, cnt, pg, status_word(cache.device).data_ptr(), qs[0], qs[1], qs[2], os_[0], os_[1], os_[2], scale, layer, n,
+              _ATTEND.pack(out.data_ptr(), q.data_ptr(), ln, cnt, pg, _STATUS_AT.get(dev) or _status_at(cache.device, dev), qs[0], qs[1], qs[2], os_[0], os_[1], os_[2], scale, layer, n,
                            heads, 1 if dtype is torch.bfloat16 else 0, 0))
         _count()
         return
@@ -354,7 +366,7 @@ def kv4_reorder(cache: KV4Cache, pages: torch.Tensor, lens: torch.Tensor, parent
     par, ln = _ints(parents, "parents", (B, K), dev), _ints(lens, "lens", (cache.slots,), dev)
     pg = _ints(pages, "pages", (cache.slots, cache.capacity // KV4_PAGE), dev)
     if dev >= 0:
-        _call(lib().llmb_kv4_reorder, "kv4_reorder", dev, cache._desc, pg, ln, par, K)
+        _call(lib().llmb_kv4_reorder, "kv4_reorder", dev, cache._desc, _REORDER.pack(pg, ln, par, K, 0))
         _count(2)
         return
     slot = torch.arange(cache.slots)
