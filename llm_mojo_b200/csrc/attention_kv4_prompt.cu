@@ -8,7 +8,9 @@
 //     and write the swizzled tiles that the tensor core reads (code x scale is exact in f16: cvt and a multiplication for two values);
 //   - the output warpgroup brings the next item's rows of q into f16's range by a power of two each (exact) and writes their tiles;
 //   - P is f16, up to 2^15: the maximum lags by up to 2^8, the rest of the range goes to small weights.
-// Rates, 16 x 12 heads, prompts of up to 1000 tokens: see DESIGN's table; the kernel for few rows (mma.sync, 32 rows a warp) takes 237 us there.
+// 16 x 12 heads, ragged prompts of up to 1000 tokens: 73 us; the kernel for few rows (mma.sync, 32 rows a warp) takes 237 us there.  All prompts
+// 1024 long: 90 us, the causal forward kernel on bf16 keys 69.  A softmax warp's chain (scores, maximum, 2^x, P) per block bounds both; the conversion
+// of the codes adds 6 us.
 #include "kv4.cuh"
 #include "attention_common.cuh"
 using namespace kv4;
@@ -144,7 +146,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) attention_kv4_prompt_kernel(con
     if (warp == 12 || warp == 15) {
       // ---------------------------------------------------------- keys (warp 12) and values (warp 15) into the ring
       // Untiled bulk copies bring a block's codes and scales (contiguous within a page) into a ring of the warp's own, three blocks ahead of their
-      // conversion; held in registers instead, they were spilled, and every block waited for its loads (145 us where this takes REPLACE).
+      // conversion; held in registers instead, they were spilled, and every block waited for its loads (145 us for the prompts above).
       const bool is_v = warp == 15;
       const uint8_t* codes = (is_v ? p.d.vc : p.d.kc) + p.layer * p.d.code_layer;
       const uint8_t* scales = (is_v ? p.d.vs : p.d.ks) + p.layer * p.d.scale_layer;
@@ -216,7 +218,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) attention_kv4_prompt_kernel(con
         issue();
       }
       if (failed)                                         // leave with no copy in flight
-        for (int x = 0; x < KP_RAW; ++x) mbar_wait(&full[x], 0);
+        for (int x = max(0, issued - KP_RAW); x < issued; ++x) mbar_wait(&full[x % KP_RAW], (x / KP_RAW) & 1);
     } else {
       // ---------------------------------------------------------- MMA issuer of lane r
       const int r = warp - 13;

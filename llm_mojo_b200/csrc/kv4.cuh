@@ -63,5 +63,5 @@ struct Kv4Attn {
   bool q_vec, o_vec;                                   // rows of q can be read 16 bytes at a time, those of out written four values at a time
 };
 
-// Rows of at least KV4_PROMPT_ROWS on the tcgen05 kernel (bf16, heads of 64): attention_kv4_prompt.cu
+// Many rows, on the tcgen05 kernel (bf16, heads of 64): attention_kv4_prompt.cu
 int kv4_attention_prompt(const Kv4Attn& p, cudaStream_t st);

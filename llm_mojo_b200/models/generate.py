@@ -113,7 +113,7 @@ class CachedDecoder:
         if tokens.numel() != self.slots:
             raise ValueError(f"one token for each of {self.slots} texts, not {tuple(tokens.shape)}")
         self._grow(1)
-        self.token.copy_(tokens.view(self.slots, 1))
+        self.token.copy_(tokens.reshape(self.slots, 1))
         self._steps += 1
         if not self.graph or self._steps == 1:                         # the first step loads kernels, which a capture may not
             return self._forward(self.token, self.cache, self.lens, None, self.pages)

@@ -69,6 +69,8 @@ class KV4Cache:
         dev, at = k_codes.device, k_codes.get_device()
         p = (k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr())
         u8 = torch.uint8
+        if p[0] == p[2] or p[1] == p[3]:
+            raise ValueError("keys and values must not be the same memory")
         if (scales != (L, S, H, T, half // 8) or v_codes.shape != codes or v_scales.shape != scales or k_scales.get_device() != at
                 or v_codes.get_device() != at or v_scales.get_device() != at or k_codes.dtype is not u8 or k_scales.dtype is not u8
                 or v_codes.dtype is not u8 or v_scales.dtype is not u8):
@@ -117,6 +119,7 @@ class KV4Cache:
 
 
 # ------------------------------------------------------------------ arguments
+# private names of torch, each with the public form beside it: the public forms take as long as a launch
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
     lambda index: torch.cuda.current_stream(index).cuda_stream
 
@@ -190,7 +193,7 @@ def _encode(x: torch.Tensor, unit: float):
     s = scale.float() * unit
     t = torch.where(s > 0, b.abs() / s, torch.zeros_like(b))
     code = sum(((t > e) if i % 2 == 0 else (t >= e)).to(torch.uint8) for i, e in enumerate((0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0)))
-    code = (code | torch.signbit(b).to(torch.uint8) << 3).flatten(-2)
+    code = torch.where(s > 0, code | torch.signbit(b).to(torch.uint8) << 3, torch.zeros_like(code)).flatten(-2)
     return code[..., 0::2] | code[..., 1::2] << 4, scale.view(torch.uint8).squeeze(-1)
 
 
@@ -353,6 +356,9 @@ def kv4_reorder(cache: KV4Cache, pages: torch.Tensor, lens: torch.Tensor, parent
     items x K = slots), in place and in every layer.  Entries of ``pages`` for whole pages and ``lens`` are permuted; of the keys and values
     only the page that is being filled is copied, at most 63 tokens.  Entries for pages that are not full name the slot itself.  A parent
     outside 0 .. K - 1 counts as j itself; lengths beyond the capacity count as the capacity.
+
+    The parents that one item names have one length, as beams that grew together have: the page in which a shorter one ends may be a full
+    page of a longer one, shared by that one's other children, and the shorter one's child goes on writing into it.
 
     A full page is never written again, so any number of slots may share it; the tokens appended next go to the slot's own place."""
     if parents.dim() != 2 or parents.numel() != cache.slots or parents.shape[1] == 0:

@@ -207,3 +207,21 @@ def test_a_row_that_is_not_finite_is_kept_as_nan_and_seen_by_no_one_else():
     out = torch.empty_like(q)
     ops.attention_kv4(out, q, c, 0, i32(6))
     assert torch.isfinite(out[0, :4]).all() and torch.isnan(out[0, 4:]).all()
+
+
+def test_keys_and_values_are_two_memories():
+    c = _cache()
+    with pytest.raises(ValueError, match="same memory"):
+        ops.KV4Cache(c.k_codes, c.k_scales, c.k_codes, c.v_scales)
+    with pytest.raises(ValueError, match="same memory"):
+        ops.KV4Cache(c.k_codes, c.k_scales, c.v_codes, c.k_scales)
+
+
+def test_a_block_too_small_for_a_scale_is_all_zeros():
+    """2^-10 is half the smallest e4m3 number, a tie that goes to zero: values of up to 6 x 2^-10 units leave neither a code nor a sign."""
+    c = _cache()
+    x = torch.full((2, 1, 2, 64), -6 * 2.0 ** -10 * c.k_unit)
+    c.k_codes.fill_(0x55)
+    ops.kv4_append(c, 0, x, x, i32(0, 3))
+    assert not c.k_codes[0, 0, :, 0].any() and not c.k_scales[0, 0, :, 0].any()
+    assert not c.k_codes[0, 1, :, 3].any() and bool((c.k_codes[0, 1, :, 4] == 0x55).all())

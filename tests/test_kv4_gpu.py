@@ -422,3 +422,19 @@ def test_the_same_inputs_give_the_same_bits():
             ops.attention_kv4(o, q, c, 0, i32([700, 33, 512]), counts=i32([n, min(n, 33), n]))
         torch.cuda.synchronize()
         assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[1][2], outs[2][2])
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+def test_blocks_around_the_smallest_scale_are_the_statement_in_pytorch(dtype):
+    """To the byte, signs of zeros too: amounts on both sides of the ties between no scale, the smallest and the next."""
+    S, H, hd = 4, 2, 64
+    x = rnd(S, 3, H, hd, dtype=torch.float32, seed=5)
+    x = (x / x.abs().unflatten(-1, (-1, 16)).amax(-1, keepdim=True).expand(S, 3, H, 4, 16).flatten(-2)).float()
+    top = torch.tensor([2.0 ** -10 * f for f in (0.5, 0.99, 1.0, 1.01, 1.5, 2.0, 2.99, 3.0, 3.01, 4.0, 5.0, 7.0)], device=DEV).view(S, 3, 1, 1)
+    x = (x * top * 6 * 2.0 ** -4).to(dtype)
+    start = [0, 5, 61, 100]
+    gpu, cpu = ops.KV4Cache.empty(1, S, H, 128, hd, DEV), ops.KV4Cache.empty(1, S, H, 128, hd, "cpu")
+    ops.kv4_append(gpu, 0, x, -x, i32(start))
+    ops.kv4_append(cpu, 0, x.cpu(), -x.cpu(), torch.tensor(start, dtype=torch.int32))
+    for name in ("k_codes", "k_scales", "v_codes", "v_scales"):
+        assert torch.equal(getattr(gpu, name).cpu(), getattr(cpu, name)), name
