@@ -516,10 +516,10 @@ int run_mma(Kv4Attn p, cudaStream_t st) {
   const long long tiles = ceil_div_ll((long long)p.n * p.group, S::ROWS), units = tiles * p.d.heads * p.d.slots;
   if (units * MOST_WARPS * 16 > 0x7fffffffLL) return LLMB_ERR_BAD_ARG;
   // How many warps share a unit.  Units that fill the chip get one warp each, or two where a second round would be a short one (256 x 16
-  // heads of 64, up to 1024 tokens: 63 us with one, 56 with two, 57 with four, 67 with eight; 1024 x 16, up to 512: 106, 112, 130, 184); fewer
-  // get up to eight, as long as all warps fit on the chip at once (32 x 12, up to 777 tokens: 16, 12.7, 11.2, 8.9; 64 x 12: 26, 23, 17, 18), and
-  // then a cluster of blocks, which costs 1 - 3 us and pays where each warp keeps three tiles (4 x 8 heads of 128, 32001 tokens: 153 us in one
-  // block, 82, 62, 37 in 2, 4, 8; 1 x 12, 1000 tokens: 5.3 in one block, 6.2 in two).
+  // heads of 64, up to 1024 tokens: 60 us with one, 54 with two, 56 with four, 68 with eight; 1024 x 16, up to 512: 106, 112, 130, 184); fewer
+  // get up to eight, as long as all warps fit on the chip at once (32 x 12, up to 777 tokens: 15.5, 12.8, 11.4, 9.1; 64 x 12: 26, 23, 17, 18), and
+  // then a cluster of blocks, which costs 1 - 3 us and pays where each warp keeps three tiles (4 x 8 heads of 128, 32001 tokens: 142 us in one
+  // block, 76, 58, 35, 49 in 2, 4, 8, 16; 1 x 12, 1000 tokens: 5.3 in one block, 6.2 in two).
   const long long fit = (long long)sm_count() * S::WARPS_SM;
   const int most = ceil_div(p.d.capacity, S::TK);
   int log_w = units > fit && units <= 2 * fit && most > 1 ? 1 : 0;
