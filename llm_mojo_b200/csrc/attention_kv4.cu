@@ -16,7 +16,8 @@ namespace {
 // and eight columns are rows of q, so that a single query pads to 8 and not to 128 (as it would in a tcgen05 product), and the codes
 // go from shared memory to registers straight into operands:
 //   K  a lane holds contiguous words of a key's row; the order of the contraction index is free as long as q is laid out alike;
-//   V  a lane holds one word (eight columns) of four keys.  cvt turns a byte into a pair of columns of one key, but the contraction runs over
+//   V  a lane holds one word (eight columns) of four keys; of the words behind a multiple of eight, a half or
+//      a quarter (64 x 16 heads of 80, up to 1024 tokens: 30.2 us with whole words, 27.9 so).  cvt turns a byte into a pair of columns of one key, but the contraction runs over
 //      keys.  With few rows (NARROW: two columns of the tile per row) the pair is contracted as it stands, against (p, 0) in a row's
 //      first column, which gives the even columns of o, and (0, p) in its second, the odd ones; with more rows two byte permutations
 //      of every four values make pairs of keys.
@@ -29,7 +30,9 @@ namespace {
 constexpr int NSTG = 2, MOST_WARPS = 8, MOST_SPLITS = 16;
 template <typename T, int HD, int NT, bool NARROW> struct MmaShape {
   static constexpr int WORDS = HD / 8, NB = HD / BLOCK, WPT = (WORDS + 3) / 4, NWV = (WORDS + 7) / 8;
-  static constexpr int TK = HD <= 64 ? 64 : 32, KS = NT == 1 ? TK : 32;         // keys of a tile; of one step of the softmax
+  static constexpr int TAIL = WORDS % 8 / 2;           // bytes of V that a lane takes where eight lanes have no word each: heads of 80, and of 32 and 96
+  // keys of a tile: as many as two stages of shared memory hold for the warps of an SM (heads of 80: 27.9 us with 32, 25.8); of one step of the softmax
+  static constexpr int TK = HD <= 96 ? 64 : 32, KS = NT == 1 ? TK : 32;
   static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1, PER_ROW = PARTS * (NARROW ? 2 : 1), ROWS = 8 * NT / PER_ROW;   // columns per row; rows of a unit
   static constexpr int CODE_BYTES = TK * HD / 2, SCALE_BYTES = TK * NB, STAGE = 2 * (CODE_BYTES + SCALE_BYTES);
   static constexpr int WARP_BYTES = NSTG * STAGE;
@@ -198,6 +201,8 @@ attention_kv4_mma_kernel(const Kv4Attn p, int log_w, int tiles) {
 #pragma unroll
         for (int y = 0; y < 4; ++y) o[i][u][t][y] = 0.f;
   }
+  auto bytes_of = [](int x) { return S::TAIL && x == NWV - 1 ? S::TAIL : 4; };          // of the x-th piece of a row of V, and where they lie
+  auto first_byte = [g](int x) { return 32 * x + (S::TAIL && x == NWV - 1 ? S::TAIL : 4) * g; };
   const int kperm = (g >> 1) + 4 * (g & 1);            // the key of row g of a tile: the keys of a lane's two columns of P^T then lie four apart in V
   const uint32_t sel_a = g & 1 ? 0x1044 : 0x4410, sel_b = g & 1 ? 0x3244 : 0x4432;      // NARROW: (p, 0) or (0, p) of the lower and the upper half
   int failed_at = -1;
@@ -350,16 +355,20 @@ attention_kv4_mma_kernel(const Kv4Attn p, int log_w, int tiles) {
         const int kv = k0 + a * 16 + j;                // this lane's keys: kv, + 4, + 8, + 12
 #pragma unroll
         for (int x = 0; x < NWV; ++x) {
-          const int w = g + 8 * x;
-          const bool in = S::WORDS % 8 == 0 || w < S::WORDS;
-          const int ws = in ? w : 0;
+          const int nu = bytes_of(x), b0 = first_byte(x);
           uint32_t hv[4][4];
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
-            const uint32_t word = *reinterpret_cast<const uint32_t*>(vc + (kv + 4 * y) * (HD / 2) + ws * 4);
-            unpack8(in ? word : 0u, hv[y]);
+            const unsigned char* at = vc + (kv + 4 * y) * (HD / 2) + b0;
+            if (nu == 4) unpack8(*reinterpret_cast<const uint32_t*>(at), hv[y]);
+            else {
+              const uint32_t bytes = nu == 2 ? *reinterpret_cast<const uint16_t*>(at) : *at;
+              hv[y][0] = e2m1x2_f16x2(bytes & 0xff);
+              hv[y][1] = nu == 2 ? e2m1x2_f16x2(bytes >> 8) : 0u;
+              hv[y][2] = hv[y][3] = 0u;
+            }
           }
-          const unsigned char* f = vs + kv * NB + (ws >> 1);
+          const unsigned char* f = vs + kv * NB + (b0 >> 3);
           // A NaN scale becomes 448 here: the key's scales are NaN as well and say so to the rows that see it, and to no other.  The same makes
           // whatever lies behind the last token a number, which its zero weight removes.
           const uint32_t s01 = min2(e4m3x2_f16x2(f[0] | (uint32_t)f[4 * NB] << 8), 0x5f005f00u), s23 = min2(e4m3x2_f16x2(f[8 * NB] | (uint32_t)f[12 * NB] << 8), 0x5f005f00u);
@@ -368,15 +377,18 @@ attention_kv4_mma_kernel(const Kv4Attn p, int log_w, int tiles) {
 #pragma unroll
             for (int y = 0; y < 4; ++y)
 #pragma unroll
-              for (int u = 0; u < 4; ++u) hv[y][u] = mul2(hv[y][u], sf[y]);
+              for (int u = 0; u < 4; ++u)
+                if (u < nu) hv[y][u] = mul2(hv[y][u], sf[y]);
 #pragma unroll
             for (int u = 0; u < NO; ++u) {
+              if (2 * u >= nu) continue;
               mma_16816(o[x][u][0], hv[0][2 * u & 3], hv[0][(2 * u + 1) & 3], hv[1][2 * u & 3], hv[1][(2 * u + 1) & 3], pf[a][0][0], pf[a][0][1]);
               mma_16816(o[x][u][0], hv[2][2 * u & 3], hv[2][(2 * u + 1) & 3], hv[3][2 * u & 3], hv[3][(2 * u + 1) & 3], pf[a][0][NARROW ? 2 : 0], pf[a][0][NARROW ? 3 : 0]);
             }
           } else {
 #pragma unroll
             for (int u = 0; u < NO; ++u) {
+              if (u >= nu) continue;
               const uint32_t a0 = mul2(__byte_perm(hv[0][u], hv[1][u], 0x5410), s01), a1 = mul2(__byte_perm(hv[0][u], hv[1][u], 0x7632), s01);
               const uint32_t a2 = mul2(__byte_perm(hv[2][u], hv[3][u], 0x5410), s23), a3 = mul2(__byte_perm(hv[2][u], hv[3][u], 0x7632), s23);
 #pragma unroll
@@ -409,11 +421,12 @@ attention_kv4_mma_kernel(const Kv4Attn p, int log_w, int tiles) {
       if (g == 0 && mine) { pm[r] = m[t][c] * cf[t][c]; pl[r] = v; }
 #pragma unroll
       for (int x = 0; x < NWV; ++x) {
-        const int w = g + 8 * x;
-        const bool in = r < rows && (S::WORDS % 8 == 0 || w < S::WORDS);
-        float* at = po + r * HD + w * 8;
+        const int nu = bytes_of(x);
+        const bool in = r < rows;
+        float* at = po + r * HD + 2 * first_byte(x);
 #pragma unroll
         for (int u = 0; u < NO; ++u) {
+          if ((NARROW ? 2 * u : u) >= nu) continue;
           const float (&y)[4] = o[x][u][t];
           if (NARROW) {                                // a byte's two columns, then the next byte's
             float4 v4 = make_float4(y[0], y[1], y[2], y[3]);
@@ -421,7 +434,8 @@ attention_kv4_mma_kernel(const Kv4Attn p, int log_w, int tiles) {
               v4.x += __shfl_xor_sync(0xffffffffu, v4.x, 1); v4.y += __shfl_xor_sync(0xffffffffu, v4.y, 1);
               v4.z += __shfl_xor_sync(0xffffffffu, v4.z, 1); v4.w += __shfl_xor_sync(0xffffffffu, v4.w, 1);
             }
-            if (in && mine) *reinterpret_cast<float4*>(at + 4 * u) = v4;
+            if (in && mine && nu == 1) *reinterpret_cast<float2*>(at) = make_float2(v4.x, v4.y);
+            else if (in && mine) *reinterpret_cast<float4*>(at + 4 * u) = v4;
           } else if (in) {
             *reinterpret_cast<float2*>(at + 2 * u) = PARTS == 1 ? make_float2(y[c], y[2 + c]) : make_float2(y[0] + y[1], y[2] + y[3]);
           }
@@ -518,14 +532,16 @@ int run_mma(Kv4Attn p, cudaStream_t st) {
   // How many warps share a unit.  Units that fill the chip get one warp each, or two where a second round would be a short one (256 x 16
   // heads of 64, up to 1024 tokens: 60 us with one, 54 with two, 56 with four, 68 with eight; 1024 x 16, up to 512: 106, 112, 130, 184); fewer
   // get up to eight, as long as all warps fit on the chip at once (32 x 12, up to 777 tokens: 15.5, 12.8, 11.4, 9.1; 64 x 12: 26, 23, 17, 18), and
-  // then a cluster of blocks, which costs 1 - 3 us and pays where each warp keeps three tiles (4 x 8 heads of 128, 32001 tokens: 142 us in one
-  // block, 76, 58, 35, 49 in 2, 4, 8, 16; 1 x 12, 1000 tokens: 5.3 in one block, 6.2 in two).
+  // then a cluster of blocks (4 x 8 heads of 128, 32001 tokens: 142 us in one block, 76, 58, 35, 49 in 2, 4, 8, 16).  The first doubling costs what
+  // joining over distributed memory does, about 1 us, and pays from two tiles a warp on; the next ones from one tile a warp on (1 x 12: 1000 tokens
+  // 5.6 in one block, 6.5 in two, 1500 6.8 and 7.5; 2000 8.1, 7.7, 6.5 in 1, 2, 4; 4000 10.3 in two, 7.7 in four; heads of 128, 1 x 8, 3000 tokens: 12.3, 8.9,
+  // 7.9 in 2, 4, 8).
   const long long fit = (long long)sm_count() * S::WARPS_SM;
   const int most = ceil_div(p.d.capacity, S::TK);
   int log_w = units > fit && units <= 2 * fit && most > 1 ? 1 : 0;
   while (log_w < 3 && (units << (log_w + 1)) <= fit && (2 << log_w) <= most) ++log_w;
   p.splits = 1;
-  if (log_w == 3) while (p.splits < MOST_SPLITS && units * 16 * p.splits <= fit && p.splits * 48 <= most) p.splits *= 2;
+  if (log_w == 3) while (p.splits < MOST_SPLITS && units * 16 * p.splits <= fit && (p.splits == 1 ? 32 : p.splits * 16) <= most) p.splits *= 2;
   const int warps = log_w == 3 ? 8 : 4;
   return launch_pdl_cluster(dim3(p.splits), kernel, dim3((unsigned)(ceil_div_ll(units << log_w, warps) * p.splits)), warps * 32, warps * S::SMEM_WARP, st, p, log_w, (int)tiles);
 }

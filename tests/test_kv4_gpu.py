@@ -438,3 +438,15 @@ def test_blocks_around_the_smallest_scale_are_the_statement_in_pytorch(dtype):
     ops.kv4_append(cpu, 0, x.cpu(), -x.cpu(), torch.tensor(start, dtype=torch.int32))
     for name in ("k_codes", "k_scales", "v_codes", "v_scales"):
         assert torch.equal(getattr(gpu, name).cpu(), getattr(cpu, name)), name
+
+
+@pytest.mark.parametrize("hd", ops.kv4.KV4_HEAD_SIZES)
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("cap,lens", [(2048, [2048, 1]), (2560, [1300, 2499]), (8192, [8192, 0]), (8192, [65, 4097])])
+def test_few_long_texts_over_many_blocks(hd, dtype, cap, lens):
+    """Capacities at which one, two and up to sixteen blocks join; lengths that leave all but one of them, or part of a tile, without keys."""
+    c, d = filled(2, 1, hd, lens, cap, dtype, seed=cap)
+    q = rnd(2, 1, 3, hd, dtype=dtype, seed=hd)
+    out = torch.empty_like(q)
+    ops.attention_kv4(out, q, c, 0, i32(lens))
+    assert_attention(out, q, d, lens, [1, 1], what=(hd, cap, lens))
