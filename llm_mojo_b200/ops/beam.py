@@ -33,7 +33,7 @@ def beam_select(scores_out: torch.Tensor, tokens: torch.Tensor, parents: torch.T
         raise ValueError(f"scores must be a contiguous fp32 [B, K], not {scores.dtype} {tuple(shape)}")
     B, K = shape
     rows, dtype = logits.shape, logits.dtype
-    if len(rows) != 2 or rows[0] != B * K or logits.get_device() != dev or (logits.stride(1) != 1 and logits.numel()):
+    if len(rows) != 2 or rows[0] != B * K or logits.get_device() != dev or (logits.stride()[1] != 1 and logits.numel()):
         raise ValueError(f"logits must be [{B * K}, at least {vocab_size}] on {_name(dev)} with dense rows, not {tuple(rows)} on {logits.device}")
     if dtype is not torch.bfloat16 and dtype is not torch.float32:
         raise TypeError(f"logits must be bf16 or fp32, not {dtype}")
@@ -75,9 +75,9 @@ def beam_select(scores_out: torch.Tensor, tokens: torch.Tensor, parents: torch.T
     if dev >= 0:
         L = lib()
         # one call's own workspace: it lives as long as the work on this stream, and captured graphs do not share it
-        work = torch.empty(n * -(-vocab_size // 4096) * (8 + 8 * K), dtype=torch.uint8, device=scores.device)
+        work = scores.new_empty(n * -(-vocab_size // 4096) * (2 + 2 * K))
         _call(L.llmb_beam_select, "beam_select", dev,
-              _SELECT.pack(so, tk, pa, fo, logits.data_ptr(), si, fi, logits.stride(0), B, K, vocab_size, eos, 1 if dtype is torch.bfloat16 else 0, 0), work.data_ptr())
+              _SELECT.pack(so, tk, pa, fo, logits.data_ptr(), si, fi, logits.stride()[0], B, K, vocab_size, eos, 1 if dtype is torch.bfloat16 else 0, 0), work.data_ptr())
         _count(2)
         return
     x = logits[:, :vocab_size].double().view(B, K, vocab_size)
