@@ -39,8 +39,6 @@ _ATTEND = struct.Struct("@6P6qf5i")          # Kv4AttendArgs of csrc/attention_k
 
 
 def _exponent(unit: float, name: str) -> int:
-    if unit == KV4_UNIT:
-        return -4
     m, e = math.frexp(unit) if isinstance(unit, (int, float)) and math.isfinite(unit) else (0.0, 0)
     if m != 0.5 or not -32 <= e - 1 <= 32:
         raise ValueError(f"{name} must be a power of two between 2^-32 and 2^32, not {unit!r}")
@@ -78,9 +76,12 @@ class KV4Cache:
                                    ("v_codes", v_codes, tuple(codes)), ("v_scales", v_scales, (L, S, H, T, half // 8))):
                 if t.dtype != u8 or t.shape != shape or t.device != dev:
                     raise ValueError(f"{name} must be uint8 {shape} on {dev}, not {t.dtype} {tuple(t.shape)} on {t.device}")
-        cs, ss = k_codes.stride(), k_scales.stride()
-        if (p[0] | p[1] | p[2] | p[3]) % 16 or not (k_codes.is_contiguous() and k_scales.is_contiguous() and v_codes.is_contiguous()
-                                                    and v_scales.is_contiguous()):
+        if (p[0] | p[1] | p[2] | p[3]) % 16 == 0 and k_codes.is_contiguous() and k_scales.is_contiguous() and v_codes.is_contiguous() and v_scales.is_contiguous():
+            cs1, ss1 = H * T * half, H * T * (half // 8)
+            cs0, ss0 = S * cs1, S * ss1
+        else:
+            cs, ss = k_codes.stride(), k_scales.stride()
+            cs0, cs1, ss0, ss1 = cs[0], cs[1], ss[0], ss[1]
             for name, t, st, ptr in (("k_codes", k_codes, cs, p[0]), ("k_scales", k_scales, ss, p[1]), ("v_codes", v_codes, cs, p[2]),
                                      ("v_scales", v_scales, ss, p[3])):
                 if t.stride() != st:
@@ -94,7 +95,8 @@ class KV4Cache:
         self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
         self.k_unit, self.v_unit = k_unit, v_unit
         self.layers, self.slots, self.kv_heads, self.capacity, self.head_size, self.device, self.index = L, S, H, T, 2 * half, dev, at
-        self._desc = _DESC.pack(*p, cs[0], cs[1], ss[0], ss[1], L, S, H, T, 2 * half, _exponent(k_unit, "k_unit"), _exponent(v_unit, "v_unit"), 0)
+        self._desc = _DESC.pack(*p, cs0, cs1, ss0, ss1, L, S, H, T, 2 * half, -4 if k_unit == KV4_UNIT else _exponent(k_unit, "k_unit"),
+                                -4 if v_unit == KV4_UNIT else _exponent(v_unit, "v_unit"), 0)
 
     @classmethod
     def empty(cls, layers: int, slots: int, kv_heads: int, max_len: int, head_size: int, device="cuda", k_unit: float = KV4_UNIT,
@@ -164,9 +166,9 @@ def _layer(cache: KV4Cache, layer: int) -> None:
         raise ValueError(f"layer {layer!r} of a cache of {cache.layers} layers")
 
 
-def _rows(t: torch.Tensor, name: str, shape: tuple, dtype, index: int) -> tuple:
-    """The strides of a tensor of rows."""
-    if t.dtype is not dtype or t.shape != shape or t.get_device() != index:
+def _rows(t: torch.Tensor, name: str, shape: tuple, dtype, index: int, known: bool = False) -> tuple:
+    """The strides of a tensor of rows (``known``: the shape and the type are the tensor's own)."""
+    if (not known and (t.dtype is not dtype or t.shape != shape)) or t.get_device() != index:
         raise ValueError(f"{name} must be {dtype} {tuple(shape)} on {_name(index)}, not {t.dtype} {tuple(t.shape)} on {t.device}")
     st = t.stride()
     if st[-1] != 1 and t.numel():
@@ -220,7 +222,7 @@ def kv4_append(cache: KV4Cache, layer: int, k: torch.Tensor, v: torch.Tensor, st
     if dtype is not torch.bfloat16 and dtype is not torch.float32:
         raise TypeError(f"k and v must be bf16 or fp32, not {dtype}")
     _layer(cache, layer)
-    ks, vs = _rows(k, "k", shape, dtype, dev), _rows(v, "v", shape, dtype, dev)
+    ks, vs = _rows(k, "k", shape, dtype, dev, True), _rows(v, "v", shape, dtype, dev)
     at, cnt = _ints(start, "start", (S,), dev), _ints(counts, "counts", (S,), dev)
     if n == 0:
         return
@@ -257,7 +259,7 @@ def kv4_values(k_out: torch.Tensor, v_out: torch.Tensor, cache: KV4Cache, layer:
         raise TypeError(f"k_out and v_out must be bf16 or fp32, not {dtype}")
     if layer is not None:
         _layer(cache, layer)
-    ks, vs = _rows(k_out, "k_out", shape, dtype, dev), _rows(v_out, "v_out", shape, dtype, dev)
+    ks, vs = _rows(k_out, "k_out", shape, dtype, dev, True), _rows(v_out, "v_out", shape, dtype, dev)
     _spread(k_out, "k_out")
     _spread(v_out, "v_out")
     if n and k_out.data_ptr() == v_out.data_ptr():
@@ -308,7 +310,7 @@ def attention_kv4(out: torch.Tensor, q: torch.Tensor, cache: KV4Cache, layer: in
     S, n, heads, hd = shape
     if not isinstance(layer, int) or not 0 <= layer < cache.layers:
         _layer(cache, layer)
-    qs, os_ = _rows(q, "q", shape, dtype, dev), _rows(out, "out", shape, dtype, dev)
+    qs, os_ = _rows(q, "q", shape, dtype, dev, True), _rows(out, "out", shape, dtype, dev)
     if not out.is_contiguous():
         _spread(out, "out")
     ln, cnt = _ints(lens, "lens", (S,), dev), _ints(counts, "counts", (S,), dev)

@@ -450,3 +450,26 @@ def test_few_long_texts_over_many_blocks(hd, dtype, cap, lens):
     out = torch.empty_like(q)
     ops.attention_kv4(out, q, c, 0, i32(lens))
     assert_attention(out, q, d, lens, [1, 1], what=(hd, cap, lens))
+
+
+def test_calls_on_two_streams_at_once_over_views_of_one_cache():
+    """Two halves of a larger cache's slots (every other one), the second of its layers, appended to and attended to on a stream each."""
+    S, H, hd, n = 6, 2, 64, 90
+    whole = ops.KV4Cache.empty(3, S, H, 192, hd, DEV)
+    views = [ops.KV4Cache(*(getattr(whole, name)[1:, i::2] for name in ("k_codes", "k_scales", "v_codes", "v_scales"))) for i in range(2)]
+    k, v = rnd(S, n, H, hd, dtype=BF, seed=1), rnd(S, n, H, hd, dtype=BF, seed=2)
+    q = rnd(S, 1, H, hd, dtype=BF, seed=3)
+    d = Dense(S, H, 192, hd, device=DEV)
+    d.append(k, v, [20] * S, [n] * S)
+    out = torch.full_like(q, 3.0)
+    lens, start = i32([110] * 3), i32([20] * 3)
+    streams = [torch.cuda.Stream() for _ in views]
+    torch.cuda.synchronize()
+    for i, (view, stream) in enumerate(zip(views, streams)):
+        with torch.cuda.stream(stream):
+            for _ in range(5):
+                ops.kv4_append(view, 0, k[i::2], v[i::2], start)
+                ops.attention_kv4(out[i::2], q[i::2], view, 0, lens)
+    torch.cuda.synchronize()
+    assert_attention(out, q, d, [110] * S, [1] * S)
+    assert not whole.k_codes[0].any() and not whole.k_codes[2].any() and bool(whole.k_codes[1].any())
