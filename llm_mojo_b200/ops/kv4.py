@@ -45,12 +45,20 @@ def _exponent(unit: float, name: str) -> int:
     return e - 1
 
 
+_STATUS_AT = {}
+
+
+def _status_at(device: torch.device, index: int) -> int:
+    at = _STATUS_AT[index] = status_word(device).data_ptr()      # the word lives as long as the process
+    return at
+
+
 class KV4Cache:
     """The four tensors of a cache (see the module), checked once.  Layers and slots may be strided views of larger caches (every third
     slot, some of the layers); heads, tokens and values lie densely, every row 16-byte aligned."""
 
     __slots__ = ("k_codes", "k_scales", "v_codes", "v_scales", "k_unit", "v_unit", "layers", "slots", "kv_heads", "capacity", "head_size",
-                 "device", "index", "_desc")
+                 "device", "index", "_desc", "_status")
 
     def __init__(self, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor,
                  k_unit: float = KV4_UNIT, v_unit: float = KV4_UNIT):
@@ -97,6 +105,8 @@ class KV4Cache:
         self.layers, self.slots, self.kv_heads, self.capacity, self.head_size, self.device, self.index = L, S, H, T, 2 * half, dev, at
         self._desc = _DESC.pack(*p, cs0, cs1, ss0, ss1, L, S, H, T, 2 * half, -4 if k_unit == KV4_UNIT else _exponent(k_unit, "k_unit"),
                                 -4 if v_unit == KV4_UNIT else _exponent(v_unit, "v_unit"), 0)
+        # made with the cache: in a call that a graph captures, the word's zeros would become a step of the graph
+        self._status = 0 if at < 0 else _STATUS_AT.get(at) or _status_at(dev, at)
 
     @classmethod
     def empty(cls, layers: int, slots: int, kv_heads: int, max_len: int, head_size: int, device="cuda", k_unit: float = KV4_UNIT,
@@ -138,14 +148,6 @@ def _call(fn, name: str, index: int, first, second) -> None:
             rc = fn(first, second, _raw_stream(index))
     if rc:
         check(rc, name)
-
-
-_STATUS_AT = {}
-
-
-def _status_at(device: torch.device, index: int) -> int:
-    at = _STATUS_AT[index] = status_word(device).data_ptr()      # the word lives as long as the process
-    return at
 
 
 def _ints(t: Optional[torch.Tensor], name: str, shape: tuple, index: int) -> int:
@@ -325,7 +327,7 @@ def attention_kv4(out: torch.Tensor, q: torch.Tensor, cache: KV4Cache, layer: in
         return
     if dev >= 0:
         _call(lib().llmb_attention_kv4, "attention_kv4", dev, cache._desc,
-              _ATTEND.pack(out.data_ptr(), q.data_ptr(), ln, cnt, pg, _STATUS_AT.get(dev) or _status_at(cache.device, dev), qs[0], qs[1], qs[2], os_[0], os_[1], os_[2], scale, layer, n,
+              _ATTEND.pack(out.data_ptr(), q.data_ptr(), ln, cnt, pg, cache._status, qs[0], qs[1], qs[2], os_[0], os_[1], os_[2], scale, layer, n,
                            heads, 1 if dtype is torch.bfloat16 else 0, 0))
         _count()
         return
