@@ -38,10 +38,11 @@ __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32
 
 // Workspace: stats [rows][chunks] float2 (maximum, sum of exponentials), lists [rows][chunks][K] of keys.
 //
-// The K-th largest of any 32 logits is no larger than the K-th largest of all.  Each warp takes that of its lanes' best, the block the largest
-// of them as a threshold; what is not below it (some forty of 4096) is ranked by counting.  Where more than CAND stay (ties, K > 32) the
-// list is taken from the registers one by one.
-constexpr int CAND = 512, RANKED = 192;
+// Each warp takes the j-th best of its lanes' best, j = K / 8 rounded up; no fewer than K logits are not below the least of the eight.  What is
+// not below it (some thirty of 4096 for K = 8) is ranked by counting.  Where more than CAND stay (ties) the list is taken from the registers one by one.
+// The largest of the warps' K-th best, the threshold before, took K rounds and left over a hundred for K = 16: 16 x 16 beams 41 us, now
+// (merge included, see there) 27.
+constexpr int CAND = 512, RANKED = THREADS;
 template <typename T, int PER>
 __global__ void __launch_bounds__(THREADS, PER == 32 ? 4 : 6) beam_chunk_kernel(float2* __restrict__ stats, unsigned long long* __restrict__ lists, const T* __restrict__ logits,
                                                              const bool* __restrict__ finished, int K, int V, long long ld, int chunks) {
@@ -73,18 +74,15 @@ __global__ void __launch_bounds__(THREADS, PER == 32 ? 4 : 6) beam_chunk_kernel(
   const float wm = warp_max(m);
   if (lane == 0) red[warp] = wm;
   uint32_t t = 0;
-  if (K <= 32) {
-    uint32_t b = mine;
-    for (int i = 0; i < K; ++i) {
-      t = __reduce_max_sync(0xffffffffu, b);
-      if (lane == __ffs(__ballot_sync(0xffffffffu, b == t)) - 1) b = 0;
-    }
+  for (int i = 0; i < K; i += WARPS) {
+    t = __reduce_max_sync(0xffffffffu, mine);
+    if (lane == __ffs(__ballot_sync(0xffffffffu, mine == t)) - 1) mine = 0;
   }
   if (lane == 0) level[warp] = t;
   __syncthreads();
   m = red[0]; t = level[0];
 #pragma unroll
-  for (int i = 1; i < WARPS; ++i) { m = fmaxf(m, red[i]); t = max(t, level[i]); }
+  for (int i = 1; i < WARPS; ++i) { m = fmaxf(m, red[i]); t = min(t, level[i]); }
   const float safe = m == -INFINITY ? 0.f : m, level_f = unordered(t);
   float2 s2 = make_float2(0.f, 0.f);
   const float2 minus = make_float2(-safe, -safe), log2e = make_float2(1.4426950408889634f, 1.4426950408889634f);
@@ -97,7 +95,7 @@ __global__ void __launch_bounds__(THREADS, PER == 32 ? 4 : 6) beam_chunk_kernel(
     if (v[j + 1] >= level_f) above |= 2u << j;
   }
   float s = s2.x + s2.y;
-  if (K > 32) above = 0xffffffffu;
+  if (t == 0) above = 0xffffffffu;                     // a warp with fewer lanes in use
   if (w != CHUNK) above &= tid < w ? (2u << (w - 1 - tid) / THREADS) - 1 : 0u;      // columns that there are
   s = warp_sum(s);
   const unsigned kept = above;
@@ -166,13 +164,17 @@ __global__ void __launch_bounds__(THREADS) beam_merge_kernel(float* __restrict__
   __shared__ float score[BEAM_MAX];
   __shared__ int kind[BEAM_MAX];                       // 0: alive, 1: finished, 2: offers nothing
   __shared__ bool fin[BEAM_MAX];
+  __shared__ unsigned long long won[BEAM_MAX];
+  __shared__ uint32_t won_flat[BEAM_MAX];
   const int item = blockIdx.x, tid = threadIdx.x, lane = tid % 32, n_lists = K * chunks;
   unsigned long long* const value = sm;                // [n_lists] ordered value of each list's head, 0: none left
   uint32_t* const flat = reinterpret_cast<uint32_t*>(sm + n_lists);      // its k V + v
-  int* const next = reinterpret_cast<int*>(flat + n_lists);              // the entry behind it
+  int* const next = reinterpret_cast<int*>(flat + n_lists);              // its beam, and the entry behind it
   unsigned long long* const stage = sm + 2 * n_lists;
   const unsigned long long* mine = lists + (long long)item * n_lists * K;
-  if (staged) for (int i = tid; i < n_lists * K; i += THREADS) stage[i] = mine[i];
+  if (staged)                                          // all in flight at once, while the log-sum-exps are made
+    for (int i = tid; i < n_lists * K; i += THREADS)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((uint32_t)__cvta_generic_to_shared(&stage[i])), "l"(mine + i) : "memory");
   for (int k = tid / 32; k < K; k += THREADS / 32) {
     const long long row = (long long)item * K + k;
     const float sc = scores[row];
@@ -195,10 +197,11 @@ __global__ void __launch_bounds__(THREADS) beam_merge_kernel(float* __restrict__
       kind[k] = !ok ? 2 : f ? 1 : l - l == 0.0 ? 0 : 2;
     }
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();
-  // entry e of list l becomes its head
-  auto advance = [&](int l, int e) {
-    const int k = l / chunks, kd = kind[k];
+  // entry e of list l, one of beam k's, becomes its head
+  auto advance = [&](int l, int k, int e) {
+    const int kd = kind[k];
     unsigned long long val = 0;
     int col = 0;
     if (e < K) {
@@ -210,36 +213,49 @@ __global__ void __launch_bounds__(THREADS) beam_merge_kernel(float* __restrict__
         val = ordered(kd == 1 && e == 0 ? (double)score[k] + 0.0 : (double)-INFINITY);
       }
     }
-    value[l] = val; flat[l] = (uint32_t)k * (uint32_t)V + (uint32_t)col; next[l] = e + 1;
+    value[l] = val; flat[l] = (uint32_t)k * (uint32_t)V + (uint32_t)col; next[l] = k << 8 | (e + 1);
   };
-  for (int l = tid; l < n_lists; l += THREADS) advance(l, 0);
+  for (int l = tid; l < n_lists; l += THREADS) advance(l, l / chunks, 0);
   __syncthreads();
   if (tid >= 32) return;
-  for (int i = 0; i < K; ++i) {
-    unsigned long long bk = 0;
-    uint32_t bi = 0xffffffffu;
-    int bl = -1;
+  // Every lane keeps the best head of its lists; the one that has the best of all takes the next of that list.  Rounds wait for one another: what can
+  // be is done behind them.
+  unsigned long long bk;
+  uint32_t bi;
+  int bl;
+  auto look = [&]() {
+    bk = 0; bi = 0xffffffffu; bl = -1;
+#pragma unroll 8
     for (int l = lane; l < n_lists; l += 32) {
       const unsigned long long x = value[l];
       if (x > bk || (x == bk && x != 0 && flat[l] < bi)) { bk = x; bi = flat[l]; bl = l; }
     }
+  };
+  look();
+  for (int i = 0; i < K; ++i) {
     const unsigned long long top = warp_max_u64(bk);
     const uint32_t idx = __reduce_min_sync(0xffffffffu, bk == top ? bi : 0xffffffffu);
     if (bl >= 0 && bk == top && bi == idx) {           // one lane: flat indexes differ
-      const int k = (int)(idx / (uint32_t)V), tok = (int)(idx - (uint32_t)k * (uint32_t)V);
-      const long long at = (long long)item * K + i;
-      scores_out[at] = (float)__longlong_as_double((long long)(top >> 63 ? top ^ (1ull << 63) : ~top));
-      tokens[at] = tok;
-      parents[at] = k;
-      if (finished_out != nullptr) finished_out[at] = tok == eos || fin[k];
-      advance(bl, next[bl]);
+      won[i] = top; won_flat[i] = idx;
+      const int n = next[bl];
+      advance(bl, n >> 8, n & 255);
+      look();
     }
     __syncwarp();
+  }
+  for (int i = lane; i < K; i += 32) {
+    const unsigned long long x = won[i];
+    const int k = (int)(won_flat[i] / (uint32_t)V), tok = (int)(won_flat[i] - (uint32_t)k * (uint32_t)V);
+    const long long at = (long long)item * K + i;
+    scores_out[at] = (float)__longlong_as_double((long long)(x >> 63 ? x ^ (1ull << 63) : ~x));
+    tokens[at] = tok;
+    parents[at] = k;
+    if (finished_out != nullptr) finished_out[at] = tok == eos || fin[k];
   }
 }
 }  // namespace
 
-// The arguments of a call as the Python side (ops/beam.py) packs them; the workspace is B K (8 + 8 K) bytes for each 4096 columns.
+// The arguments of a call as the Python side (ops/beam.py) packs them; the workspace is B K (8 + 8 K) bytes for each 8192 columns.
 struct BeamSelectArgs {
   float* scores_out; int *tokens, *parents; bool* finished_out;          // finished_out: optional
   const void* logits; const float* scores; const bool* finished;         // finished: optional
@@ -249,10 +265,11 @@ struct BeamSelectArgs {
 
 LLMB_API int llmb_beam_select(const BeamSelectArgs* a, void* work, cudaStream_t st) {
   const int K = a->K, V = a->V, rows = a->B * K;
-  // Chunks of 4096 columns; of 8192, for which a block takes two thirds of the instructions of two, where there are blocks enough (48 x 8 fp32: 34 us in
-  // chunks of 4096, 28.6 in chunks of 8192; 38 with the registers that leave two blocks on an SM instead of four).
-  const bool wide = (long long)rows * ceil_div(V, 4096) >= 2LL * sm_count() * 8;
-  const int chunks = ceil_div(V, wide ? 8192 : 4096);
+  // Chunks of 8192 columns, 4096 where that is all there are: fewer blocks with fewer lists to merge, although a chip that they do not fill waits for each
+  // of them longer (48 x 8 beams over 50257 columns, fp32: 27.7 us in chunks of 4096, 24.1 of 8192, 32.3 with the registers that leave two blocks on an SM
+  // instead of four; 1 x 4 in bf16 7.2 and 7.2, 7 x 8 14.2 and 11.3; 43 x 3 over 2044 columns 7.0 and 7.5).
+  const bool wide = V > 4096;
+  const int chunks = ceil_div(V, 8192);
   if (K < 1 || K > BEAM_MAX || rows > 65535 || (long long)K * chunks * 16 > 46 * 1024) return LLMB_ERR_BAD_ARG;
   float2* stats = (float2*)work;
   unsigned long long* lists = (unsigned long long*)(stats + (long long)rows * chunks);

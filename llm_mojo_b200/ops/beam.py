@@ -41,8 +41,8 @@ def beam_select(scores_out: torch.Tensor, tokens: torch.Tensor, parents: torch.T
         raise ValueError(f"1 to {BEAM_MAX} beams, not {K}")
     if not K <= vocab_size <= rows[1] or K * vocab_size >= 2 ** 31:
         raise ValueError(f"vocabulary of {vocab_size}: at least {K} beams, at most the {rows[1]} columns, and K x V below 2^31")
-    if B * K > 65535 or K * -(-vocab_size // 4096) > 2944:
-        raise ValueError(f"{B} items of {K} beams over {vocab_size} tokens are too many: at most 65535 rows, and K x V up to 12 million")
+    if B * K > 65535 or K * -(-vocab_size // 8192) > 2944:
+        raise ValueError(f"{B} items of {K} beams over {vocab_size} tokens are too many: at most 65535 rows, and K x V up to 24 million")
     if not -1 <= eos < vocab_size:
         raise ValueError(f"eos {eos} is no token of a vocabulary of {vocab_size}")
     if finished is not None and eos < 0:
@@ -75,7 +75,7 @@ def beam_select(scores_out: torch.Tensor, tokens: torch.Tensor, parents: torch.T
     if dev >= 0:
         L = lib()
         # one call's own workspace: it lives as long as the work on this stream, and captured graphs do not share it
-        work = scores.new_empty(n * -(-vocab_size // 4096) * (2 + 2 * K))
+        work = scores.new_empty(n * -(-vocab_size // 8192) * (2 + 2 * K))
         _call(L.llmb_beam_select, "beam_select", dev,
               _SELECT.pack(so, tk, pa, fo, logits.data_ptr(), si, fi, logits.stride()[0], B, K, vocab_size, eos, 1 if dtype is torch.bfloat16 else 0, 0), work.data_ptr())
         _count(2)

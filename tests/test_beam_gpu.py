@@ -116,3 +116,26 @@ def test_large_values_and_the_call_in_a_graph():
         g.replay()
         w = select64(logits, scores, V, None, 1)
         assert torch.equal(t.long(), w[1]) and torch.equal(p.long(), w[2])
+
+
+@pytest.mark.parametrize("B,K,V", [(3, 33, 8193), (2, 32, 40000), (9, 16, 20000), (1, 9, 130), (1, 64, 46 * 8192)])
+def test_many_beams_and_the_largest_merge(B, K, V):
+    """More lists than the merge stages, more beams than a warp has lanes, chunks whose last warps have no columns."""
+    logits = rnd(B * K, V, scale=2.5)
+    run(logits, -rnd(B, K, seed=1).abs() * 5, V)
+
+
+def test_the_same_logits_in_every_column():
+    """Every candidate of a beam ties: columns in order, however many chunks and candidates there are."""
+    B, K, V = 2, 12, 9000
+    logits = torch.full((B * K, V), 1.5, dtype=BF, device=DEV)
+    scores = -torch.arange(1, K + 1, device=DEV, dtype=FP).repeat(B, 1) * 0.25
+    so, t, p, _ = run(logits, scores, V)
+    assert torch.equal(t, torch.arange(K, device=DEV, dtype=torch.int32).repeat(B, 1)) and not p.any()
+
+
+def test_more_lists_than_the_merge_holds_are_refused():
+    K, V = 64, 46 * 8192 + 1
+    so, t, p = torch.empty(1, K, device=DEV), torch.empty(1, K, dtype=torch.int32, device=DEV), torch.empty(1, K, dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError, match="too many"):
+        ops.beam_select(so, t, p, torch.zeros(K, V, dtype=BF, device=DEV), torch.zeros(1, K, device=DEV), V)
