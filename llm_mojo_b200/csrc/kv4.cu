@@ -61,6 +61,8 @@ template <int HD> struct AppendGroup { static constexpr int value = HD <= 32 ? 4
 // The correctly rounded quotient is a midpoint only where x / s is one; a product with the rounded reciprocal is not (fl(1 / 0.875) 0.75 x 0.875
 // lies above 0.75).  It takes three operations from the correctly rounded reciprocal r (Markstein: q = x r, q + r (x - q s)), on pairs one and
 // a half; r takes one Newton step from the approximate one, which is the correctly rounded one for all eight significands that scales have.
+// The negative quotient is made (with -r for r) and the codes' signs are turned back: the correction adds a zero to q = x r = -0 and would make
+// it +0; to -q it adds one of q's sign, so that zeros keep theirs.
 // Instructions bound this kernel (about 100 for 16 values).
 template <typename T, int HD, bool VEC>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Desc d, int layer, const T* __restrict__ k, const T* __restrict__ v,
@@ -109,18 +111,19 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Desc d, int la
         float r;
         asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s32));
         r = fmaf(fmaf(-s32, r, 1.f), r, r);
-        const float2 r2 = make_float2(r, r), s2 = make_float2(-s32, -s32);
+        const float2 r2 = make_float2(-r, -r), s2 = make_float2(s32, s32);
         uint32_t code[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           float2 x = pair(w[y], j);
           if (sc == 0x7e) { x.x = fminf(fmaxf(x.x, -8.f * s32), 8.f * s32); x.y = fminf(fmaxf(x.y, -8.f * s32), 8.f * s32); }      // what saturates stays in range
-          const float2 q = __fmul2_rn(x, r2), t = __ffma2_rn(__ffma2_rn(q, s2, x), r2, q);
+          const float2 q = __fmul2_rn(x, r2), t = __ffma2_rn(__ffma2_rn(q, s2, x), r2, q);      // -x / s
           code[j] = e2m1x2(t.x, t.y);
         }
         uint2 c;
         c.x = __byte_perm(__byte_perm(code[0], code[1], 0x0040), __byte_perm(code[2], code[3], 0x0040), 0x5410);
         c.y = __byte_perm(__byte_perm(code[4], code[5], 0x0040), __byte_perm(code[6], code[7], 0x0040), 0x5410);
+        c.x ^= 0x88888888u; c.y ^= 0x88888888u;        // of x / s
         if (bad || sc == 0) c = make_uint2(0, 0);
         const long long row = (long long)head[y] * d.capacity + token[y];
         *reinterpret_cast<uint2*>(codes + row * (HD / 2)) = c;

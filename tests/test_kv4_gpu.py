@@ -473,3 +473,25 @@ def test_calls_on_two_streams_at_once_over_views_of_one_cache():
     torch.cuda.synchronize()
     assert_attention(out, q, d, [110] * S, [1] * S)
     assert not whole.k_codes[0].any() and not whole.k_codes[2].any() and bool(whole.k_codes[1].any())
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_zeros_keep_their_signs(dtype):
+    """Zeros of both signs among other values, and values so small that they round to one: the code of a negative one is 8, as in the statement
+    in PyTorch, to the byte; only a block without a scale keeps no signs."""
+    S, n, H, hd = 2, 5, 3, 64
+    x = rnd(S, n, H, hd, dtype=dtype, seed=3)
+    x[..., 0::5], x[..., 1::5] = 0.0, -0.0
+    x[..., 2::5] = -1e-30
+    x[0, 0, 0] = -0.0
+    x[1, 4, 2, :16], x[1, 4, 2, 16] = -0.0, 7.0
+    start = [0, 61]
+    gpu, cpu = ops.KV4Cache.empty(1, S, H, 128, hd, DEV), ops.KV4Cache.empty(1, S, H, 128, hd, "cpu")
+    ops.kv4_append(gpu, 0, x, -x, i32(start))
+    ops.kv4_append(cpu, 0, x.cpu(), -x.cpu(), torch.tensor(start, dtype=torch.int32))
+    for name in ("k_codes", "k_scales", "v_codes", "v_scales"):
+        assert torch.equal(getattr(gpu, name).cpu(), getattr(cpu, name)), name
+    ko, vo = torch.empty_like(x), torch.empty_like(x)
+    ops.kv4_values(ko, vo, gpu, 0, i32(start))
+    scaled = (x.unflatten(-1, (-1, 16)).abs().amax(-1, keepdim=True) > 0.01).expand(S, n, H, 4, 16).flatten(-2)
+    assert torch.equal(torch.signbit(ko), torch.signbit(x) & scaled) and torch.equal(torch.signbit(vo), ~torch.signbit(x) & scaled)
