@@ -225,3 +225,19 @@ def test_a_block_too_small_for_a_scale_is_all_zeros():
     ops.kv4_append(c, 0, x, x, i32(0, 3))
     assert not c.k_codes[0, 0, :, 0].any() and not c.k_scales[0, 0, :, 0].any()
     assert not c.k_codes[0, 1, :, 3].any() and bool((c.k_codes[0, 1, :, 4] == 0x55).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_scales_around_every_midpoint(dtype):
+    """A block's largest value on the midpoints between scales (exact in both types) and, for fp32, next to them, by the definition in 64 bits."""
+    scale = torch.arange(0, 127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    top = ((scale[1:] + scale[:-1]) / 2 * 6 * ops.kv4.KV4_UNIT).float()
+    top = torch.cat([top, torch.nextafter(top, top * 2), torch.nextafter(top, top * 0)] if dtype == torch.float32 else [top]).to(dtype)
+    x = (rnd(top.numel(), 32, seed=11).clamp(-1, 1) * top.view(-1, 1).float()).to(dtype)
+    x[:, 5::16] = -top.view(-1, 1)
+    x = x.view(1, -1, 1, 32)
+    c = ops.KV4Cache.empty(1, 1, 1, 384, 32, "cpu")
+    ops.kv4_append(c, 0, x, -x, i32(0))
+    ko, vo = torch.empty(x.shape), torch.empty(x.shape)
+    ops.kv4_values(ko, vo, c, 0, i32(0))
+    assert torch.equal(ko.double(), rounded64(x, ops.kv4.KV4_UNIT)) and torch.equal(vo, -ko)

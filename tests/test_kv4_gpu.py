@@ -495,3 +495,25 @@ def test_zeros_keep_their_signs(dtype):
     ops.kv4_values(ko, vo, gpu, 0, i32(start))
     scaled = (x.unflatten(-1, (-1, 16)).abs().amax(-1, keepdim=True) > 0.01).expand(S, n, H, 4, 16).flatten(-2)
     assert torch.equal(torch.signbit(ko), torch.signbit(x) & scaled) and torch.equal(torch.signbit(vo), ~torch.signbit(x) & scaled)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("unit", [2.0 ** -32, UNIT, 2.0 ** 20])
+def test_scales_around_every_midpoint(dtype, unit):
+    """The largest value of a block on every midpoint between two scales (five bits times six: exact in both types) and, for fp32, next to it on
+    both sides: the scale's byte, and the values, by the definition in 64 bits.  A quotient by 6 that is rounded more than once would reach the midpoint."""
+    scale = torch.arange(0, 127, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn).double()
+    top = ((scale[1:] + scale[:-1]) / 2 * 6 * unit).float()
+    top = torch.stack([top, top if dtype == BF else torch.nextafter(top, top * 2), top if dtype == BF else torch.nextafter(top, top * 0)], 1).to(dtype)
+    want = torch.bucketize(top.double() / 6 / unit, (scale[1:] + scale[:-1]) / 2)          # of equals the lower place: a tie, then
+    tie = top.double() / 6 / unit == ((scale[1:] + scale[:-1]) / 2).view(-1, 1)
+    want = torch.where(tie & (want % 2 == 1), want + 1, want)
+    x = (rnd(126, 3, 64, dtype=FP, seed=11).clamp(-1, 1) * top.unsqueeze(-1).float()).to(dtype)
+    x[..., 5::16] = -top.unsqueeze(-1)
+    x = x.view(1, -1, 1, 64)
+    c = ops.KV4Cache(*(torch.zeros(1, 1, 1, 384, w, dtype=torch.uint8, device=DEV) for w in (32, 4, 32, 4)), k_unit=unit, v_unit=unit)
+    ops.kv4_append(c, 0, x, -x, i32([0]))
+    assert torch.equal(c.k_scales[0, 0, 0, :378].long(), want.view(-1, 1).expand(378, 4)) and torch.equal(c.v_scales, c.k_scales)
+    ko, vo = (torch.empty(x.shape, device=DEV) for _ in range(2))
+    ops.kv4_values(ko, vo, c, 0, i32([0]))
+    assert torch.equal(ko.double(), rounded64(x, unit)) and torch.equal(vo, -ko)
