@@ -75,6 +75,7 @@ def run_infer_cached(model: GPT2, tokenizer: Tokenizer, prompt, gen_tokens: int,
     logits = dec.prefill([prompt])
     for t in range(gen_tokens):
         probs = ops.softmax_rows(logits, cfg.vocab_size, temperature)[0].float().cpu()
+        dec.check()
         cdf = torch.cumsum(probs, 0)
         nxt = int(min(int(torch.searchsorted(cdf, torch.tensor(rng.random_f32()), right=True)), cfg.vocab_size - 1))
         generated.append(nxt)

@@ -12,13 +12,15 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import torch
 
 from .. import ops
+from ..ops import _lib
 
 
 class CachedDecoder:
     """``slots`` texts (times ``beams``) of one model, up to ``max_len`` tokens each (the model's maximum by default).
 
     ``prefill`` takes the prompts, ``step`` one more token of every text; both return the logits behind the newest token.  On a GPU the steps are
-    replayed from a CUDA graph after the first one (``graph=False``: launched one by one)."""
+    replayed from a CUDA graph after the first one (``graph=False``: launched one by one).  Both only launch; ``check`` waits and says whether
+    what they answered is valid."""
 
     def __init__(self, model, slots: int, max_len: Optional[int] = None, beams: int = 1, graph: bool = True):
         cfg = model.config
@@ -125,6 +127,17 @@ class CachedDecoder:
         self._captured[0].replay()
         return self._captured[1]
 
+    def check(self) -> None:
+        """Raises ``KernelError`` if a kernel's bounded wait has run out since the last look: logits made since then are not valid.  Synchronises;
+        meant for places where the host waits for the device anyway."""
+        dev = self.cache.device
+        if dev.type != "cuda":
+            return
+        status = _lib.read_status(dev)
+        if status:
+            _lib.status_word(dev).zero_()
+            raise _lib.KernelError(f"a bounded device wait ran out while generating (status {status}): what was generated is not valid")
+
     def reorder(self, parents: torch.Tensor) -> None:
         """Beam j of item b becomes what beam ``parents[b, j]`` was (int32 [items, beams])."""
         if self.pages is None:
@@ -162,11 +175,16 @@ def beam_search(model, prompts: Sequence[Sequence[int]], beams: int, new_tokens:
         history[:, :, t] = tokens
         lengths = lengths.gather(1, at) + (~finished.gather(1, at)).int()
         scores, new_scores, finished, new_finished = new_scores, scores, new_finished, finished
-        if t == new_tokens - 1 or (eos >= 0 and t % 8 == 7 and bool(finished.all())):
+        last = t == new_tokens - 1
+        if not last and eos >= 0 and t % 8 == 7:
+            last = bool(finished.all())
+            dec.check()
+        if last:
             break
         if K > 1:
             dec.reorder(parents)
         logits = dec.step(tokens)
+    dec.check()
     out = []
     for row, n, s in zip(history.tolist(), lengths.tolist(), scores.double().tolist()):
         texts = [(h[:k], v) for h, k, v in zip(row, n, s)]

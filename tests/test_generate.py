@@ -162,3 +162,29 @@ def test_command_line(tmp_path):
     want = beam_search(m, [[5, 6, 7]], 3, 8)[0]
     rows = [line.split() for line in run("--beams", "3").strip().splitlines()[-3:]]
     assert [[int(t) for t in r[1:]] for r in rows] == [t for t, _ in want]
+
+
+def test_generation_asks_whether_what_it_answers_is_valid(monkeypatch):
+    """Before anything is answered, and in a long search on the way."""
+    import infer_gpt2
+    from llm_mojo_b200.ops._lib import KernelError
+    m, asked = make(), []
+
+    class Tok:
+        has_initialized, eot_token = False, 0
+    monkeypatch.setattr(CachedDecoder, "check", lambda self: asked.append(self.longest))
+    beam_search(m, [[1, 2]], 2, 20, eos=7)
+    assert asked[:2] == [2 + 7, 2 + 15] and len(asked) == 3
+    asked.clear()
+    infer_gpt2.run_infer_cached(m, Tok(), [1, 2], 3, seed=1, out=io.StringIO())
+    assert asked == [2, 3, 4]
+
+    def expired(self):
+        raise KernelError("a bounded device wait ran out")
+    monkeypatch.setattr(CachedDecoder, "check", expired)
+    out = io.StringIO()
+    with pytest.raises(KernelError):
+        beam_search(m, [[1, 2]], 2, 3)
+    with pytest.raises(KernelError):
+        infer_gpt2.run_infer_cached(m, Tok(), [1, 2], 3, seed=1, out=out)
+    assert out.getvalue() == ""

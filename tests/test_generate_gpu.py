@@ -104,3 +104,23 @@ def test_infer_writes_tokens(tmp_path):
     assert len(ids) == 12 and ids == again and all(0 <= t < 50257 for t in ids)
     best = infer_gpt2.run_beams(m, Tok(), [50256], 6, 3, out=a)
     assert len(best) == 3 and all(len(t) == 6 for t, _ in best)
+
+
+def test_a_wait_that_ran_out_is_an_error():
+    """The word that kernels set where a bounded wait ends without its event is set from the host here."""
+    import infer_gpt2
+    m = make("cuda", "bf16", WIDE, 2.0)
+    word = _lib.status_word(torch.device("cuda", torch.cuda.current_device()))
+
+    class Tok:
+        has_initialized, eot_token = False, 0
+    dec, out = CachedDecoder(m, 1), io.StringIO()
+    dec.prefill([[1, 2, 3]])
+    for call in (dec.check, lambda: beam_search(m, [[1, 2, 3], [4]], 3, 5), lambda: beam_search(m, [[1]], 2, 20, eos=7),
+                 lambda: infer_gpt2.run_infer_cached(m, Tok(), [1, 2, 3], 4, seed=3, out=out)):
+        word.fill_(1)
+        with pytest.raises(_lib.KernelError, match="wait ran out"):
+            call()
+        assert _lib.read_status() == 0                            # said once
+        assert out.getvalue() == ""                               # no token of it was written
+        call()
