@@ -139,3 +139,58 @@ def test_more_lists_than_the_merge_holds_are_refused():
     so, t, p = torch.empty(1, K, device=DEV), torch.empty(1, K, dtype=torch.int32, device=DEV), torch.empty(1, K, dtype=torch.int32, device=DEV)
     with pytest.raises(ValueError, match="too many"):
         ops.beam_select(so, t, p, torch.zeros(K, V, dtype=BF, device=DEV), torch.zeros(1, K, device=DEV), V)
+
+
+# ------------------------------------------------------------------ where chunks of 8192 columns meet
+LONG = 17000                                                 # two whole chunks and a short one
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_logits_that_are_not_finite_in_any_chunk(dtype):
+    B, K = 2, 6
+    logits = rnd(B * K, LONG + 1, dtype=dtype, scale=2.5)
+    scores = -rnd(B, K, seed=1).abs()
+    logits[0, 8192], logits[1, 16383], logits[2, 16999] = math.nan, math.inf, math.nan      # beams that offer nothing
+    logits[3, :8192] = -math.inf                             # a whole chunk ruled out: the first,
+    logits[4, 8192:16384] = -math.inf                        # the middle one,
+    logits[5, 16384:] = -math.inf                            # the last
+    logits[6, :16384] = -math.inf                            # all but the last
+    logits[7] = -math.inf
+    logits[8, 1:] = -math.inf                                # one token each, in the first, the second and the third chunk
+    logits[9], logits[9, 8192] = -math.inf, 1.0
+    logits[10], logits[10, 16999] = -math.inf, 1.0
+    run(logits, scores, LONG)
+    run(logits[6:].contiguous(), scores[:1], LONG, eos=9)
+    for at in (8191, 8192, 16384):                           # nothing but these: the others tie at -inf
+        x = torch.full((B * K, LONG), -math.inf, dtype=dtype, device=DEV)
+        x[:, at] = 1.0
+        run(x, scores, LONG)
+
+
+def test_dead_and_finished_beams_of_many_chunks():
+    B, K = 3, 4
+    logits = rnd(B * K, LONG, dtype=BF, scale=2.5)
+    scores = torch.full((B, K), -math.inf, device=DEV)
+    run(logits, scores, LONG)                                # none is alive: the lowest places
+    scores[:, 2] = 0.0                                       # one is
+    _, _, p, _ = run(logits, scores, LONG)
+    assert (p == 2).all()
+    scores = -rnd(B, K, seed=1).abs()
+    scores[0, 1], scores[1, 2] = math.nan, math.inf
+    run(logits, scores, LONG)
+    fin = torch.zeros(B, K, dtype=torch.bool, device=DEV)
+    fin[0, 1] = fin[1, 0] = fin[2, 0] = fin[2, 3] = True
+    scores[2, 0] = -math.inf
+    for eos in (0, 8191, 8192, 16999):
+        run(logits, scores, LONG, fin, eos)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_ties_across_chunks(dtype):
+    B, K = 2, 8
+    logits = rnd(B * K, LONG, dtype=dtype, scale=2.0)
+    logits[:] = logits[0]
+    logits[:, [8191, 8192, 16383, 16384, 16999, 30]] = 12.0  # of each beam, and between the beams
+    _, t, p, _ = run(logits, torch.full((B, K), -1.25, device=DEV), LONG)
+    assert t[0].tolist() == [30, 8191, 8192, 16383, 16384, 16999, 30, 8191] and p[0].tolist() == [0] * 6 + [1] * 2
+    run(torch.zeros(B * K, LONG, dtype=dtype, device=DEV), torch.zeros(B, K, device=DEV), LONG)
