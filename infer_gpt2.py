@@ -20,6 +20,7 @@ import time
 import torch
 
 from llm_mojo_b200.models import GPT2, CachedDecoder, beam_search
+from llm_mojo_b200.models.generate import on_device
 from llm_mojo_b200 import ops
 from llm_mojo_b200.utils.eval_dataloader import EvalDataLoader, eval_stat_correct
 from llm_mojo_b200.utils.sampler import SamplerRNG, sample_softmax
@@ -74,7 +75,8 @@ def run_infer_cached(model: GPT2, tokenizer: Tokenizer, prompt, gen_tokens: int,
     t0 = time.perf_counter()
     logits = dec.prefill([prompt])
     for t in range(gen_tokens):
-        probs = ops.softmax_rows(logits, cfg.vocab_size, temperature)[0].float().cpu()
+        with on_device(dec.device):
+            probs = ops.softmax_rows(logits, cfg.vocab_size, temperature)[0].float().cpu()
         dec.check()
         cdf = torch.cumsum(probs, 0)
         nxt = int(min(int(torch.searchsorted(cdf, torch.tensor(rng.random_f32()), right=True)), cfg.vocab_size - 1))
@@ -82,7 +84,7 @@ def run_infer_cached(model: GPT2, tokenizer: Tokenizer, prompt, gen_tokens: int,
         out.write(tokenizer.decode(nxt) if tokenizer.has_initialized else f"{nxt} ")
         out.flush()
         if t + 1 < gen_tokens:
-            logits = dec.step(torch.tensor([nxt], dtype=torch.int32, device=model.device))
+            logits = dec.step(torch.tensor([nxt], dtype=torch.int32, device=dec.device))
     dt = time.perf_counter() - t0
     out.write(f"\n---\n{len(generated)} tokens in {dt:.2f} s ({len(generated) / max(dt, 1e-9):.1f} tok/s)\n")
     return generated

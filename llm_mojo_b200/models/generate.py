@@ -7,12 +7,18 @@ answers does not depend on how it was cut into calls.  Linear layers run in the 
 """
 from __future__ import annotations
 
+import contextlib
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
 from .. import ops
 from ..ops import _lib
+
+
+def on_device(device: torch.device):
+    """Makes ``device`` the current one: the linear and normalisation operators launch to the current device's stream, whatever their tensors'."""
+    return torch.cuda.device(device) if device.type == "cuda" else contextlib.nullcontext()
 
 
 class CachedDecoder:
@@ -35,13 +41,14 @@ class CachedDecoder:
             raise ValueError(f"at least one text and one beam, not {slots} and {beams}")
         self.model, self.items, self.beams, self.max_len = model, slots, beams, max_len
         self.slots = slots * beams
-        self.cache = ops.KV4Cache.empty(cfg.num_layer, self.slots, cfg.num_heads, max_len, cfg.head_size, model.device)
+        self.device = model.params.device                              # with its index, whichever is current later
+        self.cache = ops.KV4Cache.empty(cfg.num_layer, self.slots, cfg.num_heads, max_len, cfg.head_size, self.device)
         self.first = self.cache.select(slice(0, None, beams))          # each item's first beam: where its prompt is read
-        self.lens = torch.zeros(self.slots, dtype=torch.int32, device=model.device)
+        self.lens = torch.zeros(self.slots, dtype=torch.int32, device=self.device)
         self.pages = self.cache.own_pages() if beams > 1 else None
         self.longest = 0                                               # of any text, known on the host
-        self.token = torch.zeros(self.slots, 1, dtype=torch.int32, device=model.device)
-        self.graph = graph and model.device.type == "cuda"
+        self.token = torch.zeros(self.slots, 1, dtype=torch.int32, device=self.device)
+        self.graph = graph and self.device.type == "cuda"
         self._captured: Optional[Tuple[torch.cuda.CUDAGraph, torch.Tensor]] = None
         self._steps = 0
 
@@ -51,10 +58,10 @@ class CachedDecoder:
         m, p, cfg = self.model, self.model.p, self.model.config
         S, n = tokens.shape
         C, NH, hd, rows = cfg.channels, cfg.num_heads, cfg.head_size, S * n
-        e = lambda *shape, dtype=m.dtype: torch.empty(*shape, dtype=dtype, device=m.device)  # noqa: E731
+        e = lambda *shape, dtype=m.dtype: torch.empty(*shape, dtype=dtype, device=self.device)  # noqa: E731
         before = lens.clone()
         lens += n if counts is None else counts
-        pos = (before.long().view(S, 1) + torch.arange(n, device=m.device)).clamp_(max=cfg.max_seq_len - 1)
+        pos = (before.long().view(S, 1) + torch.arange(n, device=self.device)).clamp_(max=cfg.max_seq_len - 1)
         x = p["wte"][tokens.long().view(-1).clamp(0, cfg.vocab_size - 1)] + p["wpe"][pos.view(-1)]        # an index from outside addresses nothing
         ln, mean, rstd, qkv, att, pre, act = e(rows, C), e(rows, dtype=torch.float32), e(rows, dtype=torch.float32), e(rows, 3 * C), e(rows, C), e(rows, 4 * C), e(rows, 4 * C)
         heads = qkv.view(S, n, 3, NH, hd)
@@ -73,7 +80,7 @@ class CachedDecoder:
             ops.matmul_fwd(nxt, act, p["fcprojw"][l], p["fcprojb"][l], residual=mid)
             x, nxt = nxt, (x if l else e(rows, C))
         if n > 1:
-            last = (counts.long() - 1 if counts is not None else torch.full((S,), n - 1, device=m.device)) + torch.arange(S, device=m.device) * n
+            last = (counts.long() - 1 if counts is not None else torch.full((S,), n - 1, device=self.device)) + torch.arange(S, device=self.device) * n
             x = x[last]
         out, logits = e(S, C), e(S, cfg.padded_vocab_size)
         ops.layernorm_fwd(out, mean[:S], rstd[:S], x, p["lnfw"], p["lnfb"])
@@ -100,12 +107,13 @@ class CachedDecoder:
         toks = torch.zeros(self.items, n, dtype=torch.int32)
         for b, t in enumerate(prompts):
             toks[b, :len(t)] = torch.tensor(list(t), dtype=torch.int32)
-        counts = torch.tensor([len(t) for t in prompts], dtype=torch.int32, device=self.model.device)
-        lens = torch.zeros(self.items, dtype=torch.int32, device=self.model.device)
-        logits = self._forward(toks.to(self.model.device), self.first, lens, None if n * self.items == sum(len(t) for t in prompts) else counts, None)
+        counts = torch.tensor([len(t) for t in prompts], dtype=torch.int32, device=self.device)
+        lens = torch.zeros(self.items, dtype=torch.int32, device=self.device)
+        with on_device(self.device):
+            logits = self._forward(toks.to(self.device), self.first, lens, None if n * self.items == sum(len(t) for t in prompts) else counts, None)
         self.lens[::self.beams] = lens
         if self.beams > 1:                                             # every beam continues its item's prompt
-            self.reorder(torch.zeros(self.items, self.beams, dtype=torch.int32, device=self.model.device))
+            self.reorder(torch.zeros(self.items, self.beams, dtype=torch.int32, device=self.device))
         return logits
 
     @torch.no_grad()
@@ -115,13 +123,17 @@ class CachedDecoder:
         if tokens.numel() != self.slots:
             raise ValueError(f"one token for each of {self.slots} texts, not {tuple(tokens.shape)}")
         self._grow(1)
+        with on_device(self.device):
+            return self._step(tokens)
+
+    def _step(self, tokens: torch.Tensor) -> torch.Tensor:
         self.token.copy_(tokens.reshape(self.slots, 1))
         self._steps += 1
         if not self.graph or self._steps == 1:                         # the first step loads kernels, which a capture may not
             return self._forward(self.token, self.cache, self.lens, None, self.pages)
         if self._captured is None:
             g = torch.cuda.CUDAGraph()
-            with torch.cuda.device(self.model.device), torch.cuda.graph(g):
+            with torch.cuda.graph(g):
                 out = self._forward(self.token, self.cache, self.lens, None, self.pages)
             self._captured = (g, out)
         self._captured[0].replay()
@@ -130,7 +142,7 @@ class CachedDecoder:
     def check(self) -> None:
         """Raises ``KernelError`` if a kernel's bounded wait has run out since the last look: logits made since then are not valid.  Synchronises;
         meant for places where the host waits for the device anyway."""
-        dev = self.cache.device
+        dev = self.device
         if dev.type != "cuda":
             return
         status = _lib.read_status(dev)
@@ -156,7 +168,7 @@ def beam_search(model, prompts: Sequence[Sequence[int]], beams: int, new_tokens:
     dec = CachedDecoder(model, len(prompts), max_len, beams, graph)
     if max(len(t) for t in prompts) + new_tokens - 1 > dec.max_len:
         raise ValueError(f"prompts of {max(len(t) for t in prompts)} tokens and {new_tokens} new ones: the cache has {dec.max_len} places")
-    cfg, dev, B, K = model.config, model.device, len(prompts), beams
+    cfg, dev, B, K = model.config, dec.device, len(prompts), beams
     if K > cfg.vocab_size:
         raise ValueError(f"{K} beams over {cfg.vocab_size} tokens")
     logits = dec.prefill(prompts).repeat_interleave(K, 0)

@@ -188,3 +188,39 @@ def test_generation_asks_whether_what_it_answers_is_valid(monkeypatch):
     with pytest.raises(KernelError):
         infer_gpt2.run_infer_cached(m, Tok(), [1, 2], 3, seed=1, out=out)
     assert out.getvalue() == ""
+
+
+def test_every_launch_is_made_with_the_models_device_current(monkeypatch):
+    """The operators without a cache among their arguments launch to the current device's stream."""
+    import contextlib
+
+    import infer_gpt2
+    from llm_mojo_b200 import ops
+    from llm_mojo_b200.models import generate
+    m, inside, launched = make(), [], []
+
+    @contextlib.contextmanager
+    def on_device(device):
+        inside.append(device)
+        yield
+        inside.pop()
+
+    def watched(fn):
+        def call(*a, **kw):
+            assert inside == [m.params.device], fn.__name__
+            launched.append(fn.__name__)
+            return fn(*a, **kw)
+        return call
+
+    class Tok:
+        has_initialized, eot_token = False, 0
+    for module in (generate, infer_gpt2):
+        monkeypatch.setattr(module, "on_device", on_device)
+    for name in ("layernorm_fwd", "matmul_fwd", "softmax_rows"):
+        monkeypatch.setattr(ops, name, watched(getattr(ops, name)))
+    dec = CachedDecoder(m, 2, beams=2)
+    dec.prefill([[1, 2], [3]])
+    dec.step(torch.zeros(4, dtype=torch.int32))
+    beam_search(m, [[1, 2]], 2, 3)
+    infer_gpt2.run_infer_cached(m, Tok(), [1, 2], 3, seed=1, out=io.StringIO())
+    assert set(launched) == {"layernorm_fwd", "matmul_fwd", "softmax_rows"} and not inside
