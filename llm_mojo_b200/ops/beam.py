@@ -14,6 +14,12 @@ BEAM_MAX = 64
 _SELECT = struct.Struct("@7Pq6i")            # BeamSelectArgs of csrc/beam.cu
 
 
+def _meets_rows(at: int, size: int, rows: int, pitch: int, width: int) -> bool:
+    """Whether the bytes at .. at + size meet one of the rows r pitch .. r pitch + width."""
+    first = max(0, (at - width) // pitch + 1) if pitch else 0          # the first row that ends behind ``at``
+    return first < rows and first * pitch < at + size and first * pitch + width > at
+
+
 def beam_select(scores_out: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, logits: torch.Tensor, scores: torch.Tensor,
                 vocab_size: int, finished_out: Optional[torch.Tensor] = None, finished: Optional[torch.Tensor] = None, eos: int = -1) -> None:
     """One step of a beam search for B items of K beams.
@@ -25,7 +31,8 @@ def beam_select(scores_out: torch.Tensor, tokens: torch.Tensor, parents: torch.T
     With ``eos``, a beam that ``finished`` (bool [B, K]) has one continuation: ``eos`` at the same score; its other candidates count -inf.
     ``finished_out`` says which of the new beams are finished: those that continue a finished one or end in ``eos``.  A beam that is not
     alive is given the score -inf (all but one of an item at the start); a beam whose score is not finite, or whose logits have no finite
-    log-sum-exp (a NaN or +inf among them, or nothing but -inf), offers -inf throughout.  Outputs may not share memory with inputs.
+    log-sum-exp (a NaN or +inf among them, or nothing but -inf), offers -inf throughout.  Outputs may not share memory with inputs (columns of
+    ``logits`` behind ``vocab_size`` are no input).
 
     The order within a beam is that of its logits, between beams that of the sums in 64 bits, with each log-sum-exp from fp32 exponentials."""
     shape, dev = scores.shape, scores.get_device()
@@ -66,6 +73,12 @@ def beam_select(scores_out: torch.Tensor, tokens: torch.Tensor, parents: torch.T
         fi, fo = (at, fo) if t is finished else (fi, at)
     if n == 0:
         return
+    xi, pitch, elt = logits.data_ptr(), logits.stride()[0], 2 if dtype is torch.bfloat16 else 4
+    pitch, width = pitch * elt, vocab_size * elt
+    end = xi + (n - 1) * pitch + width
+    for at, size in ((so, 4 * n), (tk, 4 * n), (pa, 4 * n), (fo, n if fo else 0)):
+        if at < end and at + size > xi and _meets_rows(at - xi, size, n, pitch, width):
+            raise ValueError("outputs must not share memory with the columns of logits that are read")
     spans.sort()
     end = 0
     for at, size in spans:

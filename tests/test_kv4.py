@@ -241,3 +241,32 @@ def test_scales_around_every_midpoint(dtype):
     ko, vo = torch.empty(x.shape), torch.empty(x.shape)
     ops.kv4_values(ko, vo, c, 0, i32(0))
     assert torch.equal(ko.double(), rounded64(x, ops.kv4.KV4_UNIT)) and torch.equal(vo, -ko)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_outputs_of_the_selection_are_not_among_its_logits(dtype):
+    """Each output in the columns that are read, in the last of them, across two rows; columns behind the vocabulary may hold one."""
+    B, K, V, row = 2, 3, 40, 64
+    n = B * K
+    memory = torch.zeros(n * row, dtype=dtype)
+    logits = memory.view(n, row)
+    bytes_ = memory.view(torch.uint8)
+    size = dtype.itemsize
+
+    def place(at, d):                                        # an output that starts at a byte of the logits
+        return bytes_[at:at + n * d.itemsize].view(d).view(B, K)
+
+    def call(**out):
+        o = {"scores_out": torch.empty(B, K), "tokens": torch.empty(B, K, dtype=torch.int32), "parents": torch.empty(B, K, dtype=torch.int32),
+             "finished_out": torch.empty(B, K, dtype=torch.bool), **out}
+        ops.beam_select(o.pop("scores_out"), o.pop("tokens"), o.pop("parents"), logits, torch.zeros(B, K), V, **o)
+    for name, d in (("scores_out", torch.float32), ("tokens", torch.int32), ("parents", torch.int32), ("finished_out", torch.bool)):
+        used = n * d.itemsize
+        for at in (0, 4, V * size - 4, 2 * row * size - 4, 3 * row * size - (used - 4) // 4 * 4, ((n - 1) * row + V) * size - 4):
+            with pytest.raises(ValueError, match="columns of logits"):
+                call(**{name: place(at, d)})
+        if used <= (row - V) * size:
+            call(**{name: place(V * size, d)})
+            call(**{name: place(row * size - used // 4 * 4 - (4 if used % 4 else 0), d)})
+    logits = torch.zeros(1, V, dtype=dtype).expand(n, V)     # one row for all
+    call()
