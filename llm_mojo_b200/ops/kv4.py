@@ -189,6 +189,45 @@ def _spread(t: torch.Tensor, name: str) -> None:
         span += s * (n - 1)
 
 
+def _places(t: torch.Tensor) -> list:
+    """(extent, stride in bytes) of the dimensions that have more than one index, the widest stride first."""
+    e = t.element_size()
+    return sorted(((n, s * e) for n, s in zip(t.shape, t.stride()) if n > 1), key=lambda p: -p[1])
+
+
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of one device have a byte in common; the elements of each by themselves do not overlap (see ``_spread``)."""
+    if not a.numel() or not b.numel():
+        return False
+    (da, db), e = (_places(a), _places(b)), a.element_size()
+    pa, pb = a.data_ptr(), b.data_ptr()
+    last = lambda d, t: sum((n - 1) * s for n, s in d) + t.element_size()  # noqa: E731
+    if pa >= pb + last(db, b) or pb >= pa + last(da, a):
+        return False
+    if da == db and e == b.element_size():                   # as slices of one tensor have them: a distance that indices make up, or none
+        def makes(d, far):
+            if not d:
+                return -e < far < e
+            (n, s), rest = d[0], d[1:]
+            if not s:
+                return makes(rest, far)
+            return any(makes(rest, far - i * s) for i in (far // s, far // s + 1) if -n < i < n)
+        return makes(da, pb - pa)
+    starts, width = [], []
+    for p, d, t in ((pa, da, a), (pb, db, b)):               # runs of bytes that lie densely
+        w, d = t.element_size(), list(d)
+        while d and d[-1][1] == w:
+            w *= d.pop()[0]
+        at = torch.tensor([p])
+        for n, s in d:
+            at = (at.view(-1, 1) + torch.arange(n) * s).view(-1)
+        starts.append(at)
+        width.append(w)
+    at = starts[0].sort().values
+    i = torch.searchsorted(at, starts[1] + width[1]) - 1     # the last run of a that begins before a run of b ends
+    return bool(((i >= 0) & (at[i.clamp(min=0)] + width[0] > starts[1])).any())
+
+
 # ------------------------------------------------------------------ the definitions, on any device, in fp32
 def _encode(x: torch.Tensor, unit: float):
     """(codes, scales) of x [..., head_size]: a block's scale is e4m3(amax / 6 / unit), its values e2m1(x / (scale unit)), ties to even."""
@@ -301,7 +340,7 @@ def attention_kv4(out: torch.Tensor, q: torch.Tensor, cache: KV4Cache, layer: in
     h // (heads / kv_heads).  ``lens`` [slots]: tokens in the cache; ``counts`` [slots]: how many of the n rows of a slot are queries (n without
     it).  Row i < counts[s] is the token at position lens[s] - counts[s] + i and sees the positions up to its own; a row that sees none (an
     empty slot) gives zeros; rows behind counts[s] are left as they are.  ``scale``: of the scores, 1 / sqrt(head_size) by default.
-    ``out`` may be ``q`` itself.  A page whose entry in ``pages`` names no slot gives NaN to every row that sees it.
+    ``out`` may be ``q`` itself, and otherwise has no memory in common with it.  A page whose entry in ``pages`` names no slot gives NaN to every row that sees it.
 
     Scores, statistics and sums are in fp32.  lens above the capacity count as the capacity."""
     shape, dtype, dev = q.shape, q.dtype, cache.index
@@ -313,8 +352,19 @@ def attention_kv4(out: torch.Tensor, q: torch.Tensor, cache: KV4Cache, layer: in
     if not isinstance(layer, int) or not 0 <= layer < cache.layers:
         _layer(cache, layer)
     qs, os_ = _rows(q, "q", shape, dtype, dev, True), _rows(out, "out", shape, dtype, dev)
-    if not out.is_contiguous():
+    flat = out.is_contiguous()
+    if not flat:
         _spread(out, "out")
+    qp, op = q.data_ptr(), out.data_ptr()
+    if qp != op or qs != os_:                                # rows that are written while others are still to be read
+        far, e = op - qp, 2 if dtype is torch.bfloat16 else 4
+        if flat and qs == os_:
+            near = abs(far) < q.numel() * e
+        else:
+            a, z, w = S - 1, n - 1, heads - 1
+            near = -(a * os_[0] + z * os_[1] + w * os_[2] + hd) * e < far < (a * qs[0] + z * qs[1] + w * qs[2] + hd) * e
+        if near and (far or _places(q) != _places(out)) and _meet(q, out):
+            raise ValueError(f"out must be q itself or share no memory with it (strides {qs} and {os_})")
     ln, cnt = _ints(lens, "lens", (S,), dev), _ints(counts, "counts", (S,), dev)
     pg = _ints(pages, "pages", (S, cache.capacity // KV4_PAGE), dev)
     if scale is None:
@@ -327,7 +377,7 @@ def attention_kv4(out: torch.Tensor, q: torch.Tensor, cache: KV4Cache, layer: in
         return
     if dev >= 0:
         _call(lib().llmb_attention_kv4, "attention_kv4", dev, cache._desc,
-              _ATTEND.pack(out.data_ptr(), q.data_ptr(), ln, cnt, pg, cache._status, qs[0], qs[1], qs[2], os_[0], os_[1], os_[2], scale, layer, n,
+              _ATTEND.pack(op, qp, ln, cnt, pg, cache._status, qs[0], qs[1], qs[2], os_[0], os_[1], os_[2], scale, layer, n,
                            heads, 1 if dtype is torch.bfloat16 else 0, 0))
         _count()
         return

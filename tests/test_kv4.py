@@ -270,3 +270,42 @@ def test_outputs_of_the_selection_are_not_among_its_logits(dtype):
             call(**{name: place(row * size - used // 4 * 4 - (4 if used % 4 else 0), d)})
     logits = torch.zeros(1, V, dtype=dtype).expand(n, V)     # one row for all
     call()
+
+
+def test_an_output_of_attention_is_q_itself_or_apart_from_it():
+    c = _cache(max_len=64)
+    S, n, H, hd = 2, 3, 2, 64
+    k = rnd(S, 5, H, hd)
+    ops.kv4_append(c, 0, k, k, i32(0, 0))
+    lens = i32(5, 5)
+    memory = rnd(2 * S * n * 3 * H * hd, seed=2)
+    qkv = memory[:S * n * 3 * H * hd].view(S, n, 3, H, hd)
+    q = qkv[:, :, 0]
+    want = torch.empty(S, n, H, hd)
+    ops.attention_kv4(want, q, c, 0, lens)
+    size = (S, n, H, hd)
+    one = (n * 3 * H * hd, 3 * H * hd, hd, 1)
+    for out in (memory.as_strided(size, one, 1),             # shifted by a value, a head, a token; in another order
+                memory.as_strided(size, one, hd), memory.as_strided(size, one, 3 * H * hd), memory.as_strided(size, one, n * 3 * H * hd),
+                memory.as_strided(size, (n * H * hd, H * hd, hd, 1), 0), memory.as_strided(size, (hd, S * H * hd, S * hd, 1), 64),
+                memory.as_strided(size, (3 * H * hd, S * 3 * H * hd, hd, 1), 0)):
+        with pytest.raises(ValueError, match="q itself"):
+            ops.attention_kv4(out, q, c, 0, lens)
+    with pytest.raises(ValueError, match="q itself"):        # rows of q that are one
+        x = memory[:S * n * H * hd].view(size)
+        ops.attention_kv4(x, x[:, :1].expand(size), c, 0, lens)
+    kept = q.clone()
+    for out in (qkv[:, :, 1], qkv[:, :, 2]):                 # the places of the keys and values, which are in the cache by now
+        ops.attention_kv4(out, q, c, 0, lens)
+        assert torch.equal(out, want) and torch.equal(q, kept)
+    wide = torch.zeros(S, n, H, 2 * hd)                      # halves of one row, with other strides from token to token
+    wide[..., :hd] = kept
+    ops.attention_kv4(wide[..., hd:], wide[..., :hd], c, 0, lens)
+    assert torch.equal(wide[..., hd:], want)
+    row = torch.zeros(S, n, 2 * H * hd)
+    row[..., :H * hd] = kept.flatten(-2)
+    out = row.as_strided(size, (n * 2 * H * hd, 2 * H * hd, hd, 1), H * hd)
+    ops.attention_kv4(out, row[..., :H * hd].view(size), c, 0, lens)
+    assert torch.equal(out, want)
+    ops.attention_kv4(q, q, c, 0, lens)
+    assert torch.equal(q, want)
