@@ -303,7 +303,8 @@ def kv4_values(k_out: torch.Tensor, v_out: torch.Tensor, cache: KV4Cache, layer:
     ks, vs = _rows(k_out, "k_out", shape, dtype, dev, True), _rows(v_out, "v_out", shape, dtype, dev)
     _spread(k_out, "k_out")
     _spread(v_out, "v_out")
-    if n and k_out.data_ptr() == v_out.data_ptr():
+    kp, vp = k_out.data_ptr(), v_out.data_ptr()
+    if (abs(kp - vp) < k_out.numel() * (2 if dtype is torch.bfloat16 else 4) or not (k_out.is_contiguous() and v_out.is_contiguous())) and _meet(k_out, v_out):
         raise ValueError("k_out and v_out are two outputs: they must not be the same memory")
     if layer is None and n and ks != vs:
         raise ValueError(f"k_out and v_out must have the same strides, not {ks} and {vs}")
@@ -312,7 +313,7 @@ def kv4_values(k_out: torch.Tensor, v_out: torch.Tensor, cache: KV4Cache, layer:
         return
     if dev >= 0:
         _call(lib().llmb_kv4_values, "kv4_values", dev, cache._desc,
-              _VALUES.pack(k_out.data_ptr(), v_out.data_ptr(), at, pg, ks[0] if layer is None else 0, ks[-4], ks[-3], ks[-2], vs[-4], vs[-3], vs[-2],
+              _VALUES.pack(kp, vp, at, pg, ks[0] if layer is None else 0, ks[-4], ks[-3], ks[-2], vs[-4], vs[-3], vs[-2],
                            -1 if layer is None else layer, n, 1 if dtype is torch.bfloat16 else 0, 0))
         _count()
         return

@@ -309,3 +309,20 @@ def test_an_output_of_attention_is_q_itself_or_apart_from_it():
     assert torch.equal(out, want)
     ops.attention_kv4(q, q, c, 0, lens)
     assert torch.equal(q, want)
+
+
+def test_the_two_read_backs_share_no_memory():
+    c = _cache()
+    memory, size = torch.zeros(2 * 3 * 2 * 2 * 64), (2, 3, 2, 64)
+    pair = memory.view(2, 3, 2, 2, 64)
+    k, v = rnd(2, 3, 2, 64), rnd(2, 3, 2, 64, seed=1)
+    ops.kv4_append(c, 0, k, v, i32(0, 0))
+    ops.kv4_values(pair[:, :, 0], pair[:, :, 1], c, 0, i32(0, 0))            # side by side in one tensor
+    assert torch.equal(pair[:, :, 0].double(), rounded64(k, c.k_unit)) and torch.equal(pair[:, :, 1].double(), rounded64(v, c.v_unit))
+    flat = memory[:2 * 3 * 2 * 64].view(size)
+    for shift in (1, 64, 2 * 64, 3 * 2 * 64):
+        for a, b in ((flat, memory[shift:shift + flat.numel()].view(size)), (memory[shift:shift + flat.numel()].view(size), flat),
+                     (pair[:, :, 0], memory[shift:shift + flat.numel()].view(size))):
+            with pytest.raises(ValueError, match="same memory"):
+                ops.kv4_values(a, b, c, 0, i32(0, 0))
+    ops.kv4_values(flat[:, :0], flat[:, :0], c, 0, i32(0, 0))                # nothing to write is no error
