@@ -15,6 +15,7 @@ CUDA tensors run ``csrc/kv4.cu`` and ``csrc/attention_kv4.cu``; CPU tensors run 
 """
 from __future__ import annotations
 
+import itertools
 import math
 import struct
 from typing import Optional
@@ -87,6 +88,7 @@ class KV4Cache:
         if (p[0] | p[1] | p[2] | p[3]) % 16 == 0 and k_codes.is_contiguous() and k_scales.is_contiguous() and v_codes.is_contiguous() and v_scales.is_contiguous():
             cs1, ss1 = H * T * half, H * T * (half // 8)
             cs0, ss0 = S * cs1, S * ss1
+            c, s, dense = L * cs0, L * ss0, True
         else:
             cs, ss = k_codes.stride(), k_scales.stride()
             cs0, cs1, ss0, ss1 = cs[0], cs[1], ss[0], ss[1]
@@ -100,6 +102,11 @@ class KV4Cache:
                 row = H * T * c
                 if (S > 1 and st[1] < row) or (L > 1 and st[0] < row) or (L > 1 and S > 1 and (S - 1) * st[1] + row > st[0] and (L - 1) * st[0] + row > st[1]):
                     raise ValueError(f"{name}: slots and layers must not overlap (strides {st})")
+            c, s, dense = (L - 1) * cs0 + (S - 1) * cs1 + H * T * half, (L - 1) * ss0 + (S - 1) * ss1 + H * T * (half // 8), False
+        kc, ks, vc, vs = p                                   # c, s: from the first byte of codes and of scales to their last
+        if (-c < kc - vc < c or -s < ks - vs < s or -s < ks - kc < c or -s < vs - kc < c or -s < ks - vc < c or -s < vs - vc < c) and (
+                dense or any(_meet(a, b) for a, b in itertools.combinations((k_codes, k_scales, v_codes, v_scales), 2))):
+            raise ValueError("codes and scales of keys and of values are four tensors: they must not share memory")
         self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
         self.k_unit, self.v_unit = k_unit, v_unit
         self.layers, self.slots, self.kv_heads, self.capacity, self.head_size, self.device, self.index = L, S, H, T, 2 * half, dev, at

@@ -326,3 +326,28 @@ def test_the_two_read_backs_share_no_memory():
             with pytest.raises(ValueError, match="same memory"):
                 ops.kv4_values(a, b, c, 0, i32(0, 0))
     ops.kv4_values(flat[:, :0], flat[:, :0], c, 0, i32(0, 0))                # nothing to write is no error
+
+
+def test_the_four_tensors_of_a_cache_share_no_memory():
+    L, S, H, T, half = 2, 3, 2, 64, 32
+    nc, ns = L * S * H * T * half, L * S * H * T * half // 8
+    memory = torch.zeros(8 * nc, dtype=torch.uint8)
+    codes = lambda at: memory[at:at + nc].view(L, S, H, T, half)  # noqa: E731
+    scales = lambda at: memory[at:at + ns].view(L, S, H, T, half // 8)  # noqa: E731
+    ops.KV4Cache(codes(0), scales(2 * nc), codes(nc), scales(2 * nc + ns))               # one behind the other
+    for at in ((0, 4 * nc, 16, 5 * nc), (nc, 4 * nc, 16, 5 * nc), (0, 4 * nc, nc - 16, 5 * nc), (0, nc - 16, 2 * nc, 5 * nc), (0, 4 * nc, 2 * nc, nc - 16),
+               (0, 4 * nc, 2 * nc, 3 * nc - 16), (ns - 16, 0, 2 * nc, 5 * nc), (0, 4 * nc, 2 * nc, 4 * nc + ns - 16), (0, 2 * nc + 64, 2 * nc, 5 * nc)):
+        with pytest.raises(ValueError, match="share memory"):
+            ops.KV4Cache(codes(at[0]), scales(at[1]), codes(at[2]), scales(at[3]))
+    # keys and values of each layer, and of each slot, side by side in one tensor: no byte in common
+    x, y = torch.zeros(L, 2, S, H, T, half, dtype=torch.uint8), torch.zeros(L, S, 2, H, T, half // 8, dtype=torch.uint8)
+    c = ops.KV4Cache(x[:, 0], y[:, :, 0], x[:, 1], y[:, :, 1])
+    k, v = rnd(S, 5, H, 2 * half), rnd(S, 5, H, 2 * half, seed=1)
+    ops.kv4_append(c, 1, k, v, i32(0, 3, 60))
+    ko, vo = torch.empty_like(k), torch.empty_like(v)
+    ops.kv4_values(ko, vo, c, 1, i32(0, 3, 60))
+    assert torch.equal(ko[:2].double(), rounded64(k, c.k_unit)[:2]) and torch.equal(vo[:2].double(), rounded64(v, c.v_unit)[:2])
+    with pytest.raises(ValueError, match="share memory"):
+        ops.KV4Cache(x[:, 0], y[:, :, 0], x[:, 0, :].as_strided((L, S, H, T, half), x[:, 0].stride(), 64), y[:, :, 1])
+    with pytest.raises(ValueError, match="share memory"):
+        ops.KV4Cache(x[:, 0], y[:, :, 0], x[:, 1], y.as_strided(y[:, :, 0].shape, y[:, :, 0].stride(), 16))
