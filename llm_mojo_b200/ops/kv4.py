@@ -433,6 +433,9 @@ def kv4_reorder(cache: KV4Cache, pages: torch.Tensor, lens: torch.Tensor, parent
         raise ValueError("kv4_reorder permutes pages and lens: both are needed")
     par, ln = _ints(parents, "parents", (B, K), dev), _ints(lens, "lens", (cache.slots,), dev)
     pg = _ints(pages, "pages", (cache.slots, cache.capacity // KV4_PAGE), dev)
+    tables, each = 4 * pages.numel(), 4 * cache.slots        # bytes, of lens and of parents alike
+    if -each < ln - par < each or -tables < pg - par < each or -tables < pg - ln < each:
+        raise ValueError("pages, lens and parents must not share memory")
     if dev >= 0:
         _call(lib().llmb_kv4_reorder, "kv4_reorder", dev, cache._desc, _REORDER.pack(pg, ln, par, K, 0))
         _count(2)

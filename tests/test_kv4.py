@@ -351,3 +351,14 @@ def test_the_four_tensors_of_a_cache_share_no_memory():
         ops.KV4Cache(x[:, 0], y[:, :, 0], x[:, 0, :].as_strided((L, S, H, T, half), x[:, 0].stride(), 64), y[:, :, 1])
     with pytest.raises(ValueError, match="share memory"):
         ops.KV4Cache(x[:, 0], y[:, :, 0], x[:, 1], y.as_strided(y[:, :, 0].shape, y[:, :, 0].stride(), 16))
+
+
+def test_tables_of_a_reorder_share_no_memory():
+    c = _cache(slots=6, max_len=128)
+    memory = torch.zeros(40, dtype=torch.int32)
+    at = lambda i, *shape: memory[i:i + math.prod(shape)].view(shape)  # noqa: E731
+    ops.kv4_reorder(c, at(6, 6, 2), at(0, 6), at(18, 2, 3))                  # side by side
+    ops.kv4_reorder(c, at(12, 6, 2), at(24, 6), at(6, 2, 3))
+    for pages, lens, parents in ((0, 11, 20), (5, 0, 20), (0, 20, 11), (9, 20, 4), (20, 0, 5), (20, 5, 0), (20, 0, 0)):
+        with pytest.raises(ValueError, match="share memory"):
+            ops.kv4_reorder(c, at(pages, 6, 2), at(lens, 6), at(parents, 2, 3))
