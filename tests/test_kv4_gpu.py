@@ -517,3 +517,37 @@ def test_scales_around_every_midpoint(dtype, unit):
     ko, vo = (torch.empty(x.shape, device=DEV) for _ in range(2))
     ops.kv4_values(ko, vo, c, 0, i32([0]))
     assert torch.equal(ko.double(), rounded64(x, unit)) and torch.equal(vo, -ko)
+
+
+@pytest.mark.parametrize("S,heads,kv_heads,n,ragged,paged", [
+    (16, 12, 12, 320, True, False),                          # three tiles: two that share a stream of keys, and one beside an empty one
+    (16, 12, 12, 320, True, True),
+    (40, 12, 3, 100, True, False),                           # rows of four heads over one
+    (160, 2, 2, 300, True, True),                            # more pairs of tiles than are sorted by their cost
+    (160, 2, 2, 300, False, False),
+    (9, 20, 20, 384, False, True),
+])
+def test_prompts_of_more_items_than_the_chip_has_places(S, heads, kv_heads, n, ragged, paged):
+    """Each block of the kernel for prompts takes several items in turn: texts that see nothing, have no rows, rows in one tile of two or one row in
+    the second, fewer keys than rows; a capacity that ends inside a block of 128 keys.  The same bits every time."""
+    hd, T = 64, 832
+    tiles = -(-n * heads // kv_heads // 128)
+    assert -(-tiles // 2) * kv_heads * S > torch.cuda.get_device_properties(0).multi_processor_count      # or a block has no second item
+    kinds = [(n + 400, n), (0, n), (n // 2, n), (n + 7, 0), (T, 1), (T, n), (n + 130, 129 * kv_heads // heads + 1), (n, 128 * kv_heads // heads), (n, n)]
+    lens, counts = zip(*(kinds[(5 * s + s // 9) % 9] for s in range(S)))
+    lens, counts = [min(x, T) for x in lens], list(counts) if ragged else [n] * S
+    c, d = filled(S, kv_heads, hd, lens, T)
+    pages = None
+    if paged:                                                # any page of any text: what lies there is read as it is
+        pages = torch.randint(0, S, (S, T // 64), generator=torch.Generator().manual_seed(4)).to(torch.int32)
+        e = Dense(S, kv_heads, T, hd, device=DEV)
+        at = pages.to(DEV).long().repeat_interleave(64, 1), torch.arange(T, device=DEV)
+        e.k, e.v = d.k[at], d.v[at]
+        d, pages = e, pages.to(DEV)
+    q = rnd(S, n, heads, hd, dtype=BF, seed=5)
+    outs = [torch.full_like(q, 3.0) for _ in range(3)]
+    for out in outs:
+        ops.attention_kv4(out, q, c, 0, i32(lens), counts=i32(counts) if ragged else None, pages=pages)
+    assert_attention(outs[0], q, d, lens, counts)
+    assert all((outs[0][s, k:] == 3.0).all() for s, k in enumerate(counts))
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2]) and _lib.read_status() == 0
