@@ -545,13 +545,22 @@ int run_mma(Kv4Attn p, cudaStream_t st) {
   const int warps = log_w == 3 ? 8 : 4;
   return launch_pdl_cluster(dim3(p.splits), kernel, dim3((unsigned)(ceil_div_ll(units << log_w, warps) * p.splits)), warps * 32, warps * S::SMEM_WARP, st, p, log_w, (int)tiles);
 }
-// Rows of a key head from which the tcgen05 kernel is the faster one (its tile has 128): 16 x 12 heads, 64 rows behind nothing 12.3 us where
-// the kernel above takes 28.7, behind 700 tokens 31.4 and 34.3; 32 rows behind 700 tokens 31 and 20.
-constexpr int PROMPT_ROWS = 64;
+// The tcgen05 kernel takes calls of PROMPT_ROWS rows of a key head and more, if its items (a tile of 128 rows, or two where there are more tiles
+// than SMs, of one slot and key head) occupy three fifths of the SMs or the cache is short.  It does not share an item's keys between blocks; the
+// kernel above does, and is the faster one where few items have many keys: 64 rows of 1 x 12 heads behind 1000, 8000 and 30000 tokens 20, 109, 390 us
+// there and 15, 22, 51 here, one token of 64 heads over one with 30000 tokens 384 and 25; 128 rows of 8 x 16 behind 4000 63 there and 94 here.
+// Short caches (up to PROMPT_SHORT tokens) take 7.2 us there and 10.9 here (1 x 12, 64 rows), 500 tokens of 64 heads over one 11.8 and 9.7.
+// In 551 calls of 64 to 1024 rows the rule is 1.6 % from the faster kernel's time; what it misses are tiles of 64 to 96 rows on a full chip
+// (16 x 12, 64 rows behind 700 tokens: 32 there and 26 here).
+constexpr int PROMPT_ROWS = 64, PROMPT_SHORT = 384;
 template <typename T, int HD>
 int run(const Kv4Attn& p, cudaStream_t st) {
   const long long rows = (long long)p.n * p.group;
-  if (sizeof(T) == 2 && HD == 64 && rows >= PROMPT_ROWS) return kv4_attention_prompt(p, st);
+  if (sizeof(T) == 2 && HD == 64 && rows >= PROMPT_ROWS) {
+    const long long units = (long long)p.d.slots * p.d.heads, tiles = ceil_div_ll(rows, 128);
+    const long long items = units * (tiles * units <= sm_count() ? tiles : ceil_div_ll(tiles, 2));
+    if (items * 5 >= sm_count() * 3LL || p.d.capacity <= PROMPT_SHORT) return kv4_attention_prompt(p, st);
+  }
   constexpr int R8 = sizeof(T) == 4 ? 4 : 8, MOST = HD <= 64 ? 4 : 2;
   if (rows <= R8 / 2) return run_mma<T, HD, 1, true>(p, st);
   if (rows <= R8) return run_mma<T, HD, 1, false>(p, st);

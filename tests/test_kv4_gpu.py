@@ -551,3 +551,33 @@ def test_prompts_of_more_items_than_the_chip_has_places(S, heads, kv_heads, n, r
     assert_attention(outs[0], q, d, lens, counts)
     assert all((outs[0][s, k:] == 3.0).all() for s, k in enumerate(counts))
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2]) and _lib.read_status() == 0
+
+
+def test_many_query_heads_over_a_long_text_share_its_keys():
+    """Sixty and sixty-four query heads over one key head are the same work: no form of the operator may leave a long text to a single block.
+    (It took sixteen times as long; four is far from both.)"""
+    c = ops.KV4Cache.empty(1, 1, 1, 30016, 64, DEV)
+    d = Dense(1, 1, 30016, 64, device=DEV)
+    k, v = rnd(1, 3000, 1, 64, dtype=BF), rnd(1, 3000, 1, 64, dtype=BF, seed=1)
+    for at in range(0, 30000, 3000):
+        ops.kv4_append(c, 0, k.roll(at // 3000, 1), v, i32([at]))
+        d.append(k.roll(at // 3000, 1), v, [at], [3000])
+    took = {}
+    for heads in (60, 64):
+        q = rnd(1, 1, heads, 64, dtype=BF, seed=heads)
+        out = torch.empty_like(q)
+        graph = torch.cuda.CUDAGraph()
+        ops.attention_kv4(out, q, c, 0, i32([30000]))
+        lens = i32([30000])
+        with torch.cuda.graph(graph):
+            for _ in range(20):
+                ops.attention_kv4(out, q, c, 0, lens)
+        graph.replay()
+        a, z = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        graph.replay()
+        z.record()
+        z.synchronize()
+        took[heads] = a.elapsed_time(z)
+        assert_attention(out, q, d, [30000], [1])
+    assert took[64] < 4 * took[60], took
