@@ -581,3 +581,75 @@ def test_many_query_heads_over_a_long_text_share_its_keys():
         took[heads] = a.elapsed_time(z)
         assert_attention(out, q, d, [30000], [1])
     assert took[64] < 4 * took[60], took
+
+
+def assert_lagging_attention(got, q, dense, lens, counts, scale=None, what=""):
+    """``assert_attention`` for bf16 and a maximum that may lag.  A row's weights are 2^(7 + s - m) for the largest score m of some keys that the row
+    has seen, so that the weight of that key is 2^7 and the sum of all at least as much.  A weight is rounded to f16: by 2^-11 of itself, or, below
+    f16's smallest normal number, by half of 2^-24.  That is 2^-25 / 2^7 = 2^-32 of the sum for each key, whatever the other weights: 2^-32 sum |v|
+    beside the terms of ``assert_attention``, which takes the largest weight for 2^13 and more."""
+    want, mag = attention64(q, dense, lens, counts, scale)
+    S, n, heads, hd = q.shape
+    group, sc = heads // dense.k.shape[2], 1 / math.sqrt(hd) if scale is None else abs(scale)
+    for s in range(S):
+        c, L = counts[s], min(lens[s], dense.T)
+        w, g = want[s, :c], got[s, :c].double()
+        assert torch.equal(torch.isnan(g), torch.isnan(w)), (what, s)
+        k, v = (x[s, :L].nan_to_num(0.0).abs().repeat_interleave(group, 1) for x in (dense.k, dense.v))
+        qk = (q[s, :c].double().abs().nan_to_num(0.0) * (k.amax(0) if L else 0.0)).sum(-1) * sc
+        delta = 2.0 ** -10 + 2 * (hd + 8) * 2.0 ** -24 * qk + 2.0 ** -22 * qk + (L / 16 + 80) * 2.0 ** -23
+        tol = 2.0 ** -8 * w.abs() + delta.unsqueeze(-1) * mag[s, :c] + 2.0 ** -32 * v.sum(0) + 1e-30
+        off = ((g - w).abs() - tol).nan_to_num(-1.0)
+        assert not off.numel() or off.max().item() <= 0, (what, s, off.max().item())
+
+
+@pytest.mark.parametrize("T", [320, 832])
+def test_prompts_on_the_tensor_memory_kernel(T):
+    """Sixteen texts of twelve heads, 200 rows: in place among packed values, through strides at odd addresses, with extreme scales, queries, values
+    and pages that are not finite, and bytes behind the last token."""
+    S, H, hd, n = 16, 12, 64, 200
+    lens = [T - 17 * (s % 4) if s % 3 else n + s for s in range(S)]
+    c, d = filled(S, H, hd, lens, T)
+    for byte in (0xff, 0x7e):                                # behind the last token: NaN, the largest
+        for s in range(S):
+            for t in (c.k_scales, c.v_scales, c.k_codes, c.v_codes):
+                t[:, s, :, lens[s]:] = byte
+    qkv = rnd(S, n, 3, H, hd, dtype=BF, seed=5)
+    q, rest = qkv[:, :, 0], qkv[:, :, 1:].clone()
+    ref = q.clone()
+    for scale in (None, -0.3, 0.0, 1e3):
+        q.copy_(ref if scale != 1e3 else ref * 1e-3)
+        want = q.clone()
+        ops.attention_kv4(q, q, c, 0, i32(lens), scale=scale)
+        assert_lagging_attention(q, want, d, lens, [n] * S, scale=scale, what=scale)
+        assert torch.equal(qkv[:, :, 1:], rest)
+    buf = torch.zeros(H * S * n * (hd + 3) + 1, dtype=BF, device=DEV)[1:].view(H, S, n, hd + 3)
+    odd = torch.empty(S * n * H * hd + 1, dtype=BF, device=DEV)[1:].view(S, n, H, hd)
+    odd.copy_(ref)
+    out = buf[..., :hd].permute(1, 2, 0, 3)
+    ops.attention_kv4(out, odd, c, 0, i32(lens))
+    assert_lagging_attention(out, odd, d, lens, [n] * S)
+    assert (buf[..., hd:] == 0).all()
+    # a query that is not finite spoils its own row; a key or value its token and head, for those that see it
+    odd[3, 7, 2, 5], odd[9, 199, 11, 0] = math.nan, math.inf
+    ops.attention_kv4(out, odd, c, 0, i32(lens))
+    bad = torch.zeros(S, n, H, dtype=torch.bool, device=DEV)
+    bad[3, 7, 2] = bad[9, 199, 11] = True
+    assert torch.equal(~torch.isfinite(out).all(-1), bad)
+    x, y = rnd(S, 1, H, hd, dtype=BF, seed=7), rnd(S, 1, H, hd, dtype=BF, seed=8)
+    x[:, :, 1, 3], y[:, :, 4, 17] = math.nan, math.inf
+    at = [L - n // 2 for L in lens]
+    ops.kv4_append(c, 0, x, y, i32(at))
+    d.append(x, y, at, [1] * S)
+    ops.attention_kv4(out, ref, c, 0, i32(lens))
+    assert_lagging_attention(out, ref, d, lens, [n] * S)
+    assert torch.isnan(out[:, -1, 1]).all() and torch.isnan(out[:, -1, 4]).all() and torch.isfinite(out[:, :n // 2]).all()
+    pages = c.own_pages()
+    pages[2, 1], pages[5, 4] = -1, S                         # tokens 64 .. 127 of one text, 256 .. 319 of another
+    c, d = filled(S, H, hd, lens, T, seed=3)
+    ops.attention_kv4(out, ref, c, 0, i32(lens), pages=pages)
+    pos = i32(lens).view(S, 1) - n + torch.arange(n, device=DEV)
+    bad = torch.zeros(S, n, dtype=torch.bool, device=DEV)
+    bad[2], bad[5] = pos[2] >= 64, pos[5] >= 256
+    assert torch.equal(torch.isnan(out).all(-1).all(-1), bad) and torch.equal(torch.isnan(out).any(-1).any(-1), bad)
+    assert _lib.read_status() == 0
