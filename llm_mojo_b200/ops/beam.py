@@ -73,24 +73,23 @@ def beam_select(scores_out: torch.Tensor, tokens: torch.Tensor, parents: torch.T
         fi, fo = (at, fo) if t is finished else (fi, at)
     if n == 0:
         return
-    xi, pitch, elt = logits.data_ptr(), logits.stride()[0], 2 if dtype is torch.bfloat16 else 4
-    pitch, width = pitch * elt, vocab_size * elt
-    end = xi + (n - 1) * pitch + width
-    for at, size in ((so, 4 * n), (tk, 4 * n), (pa, 4 * n), (fo, n if fo else 0)):
-        if at < end and at + size > xi and _meets_rows(at - xi, size, n, pitch, width):
-            raise ValueError("outputs must not share memory with the columns of logits that are read")
     spans.sort()
     end = 0
     for at, size in spans:
         if at < end:
             raise ValueError("outputs must not share memory with each other or with inputs")
         end = at + size
+    xi, pitch, elt = logits.data_ptr(), logits.stride()[0], 2 if dtype is torch.bfloat16 else 4
+    if spans[0][0] < xi + ((n - 1) * pitch + vocab_size) * elt and end > xi:
+        for at, size in ((so, 4 * n), (tk, 4 * n), (pa, 4 * n), (fo, n if fo else 0)):
+            if size and _meets_rows(at - xi, size, n, pitch * elt, vocab_size * elt):
+                raise ValueError("outputs must not share memory with the columns of logits that are read")
     if dev >= 0:
         L = lib()
         # one call's own workspace: it lives as long as the work on this stream, and captured graphs do not share it
         work = scores.new_empty(n * -(-vocab_size // 8192) * (2 + 2 * K))
         _call(L.llmb_beam_select, "beam_select", dev,
-              _SELECT.pack(so, tk, pa, fo, logits.data_ptr(), si, fi, logits.stride()[0], B, K, vocab_size, eos, 1 if dtype is torch.bfloat16 else 0, 0), work.data_ptr())
+              _SELECT.pack(so, tk, pa, fo, xi, si, fi, pitch, B, K, vocab_size, eos, 1 if dtype is torch.bfloat16 else 0, 0), work.data_ptr())
         _count(2)
         return
     x = logits[:, :vocab_size].double().view(B, K, vocab_size)

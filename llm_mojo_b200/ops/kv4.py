@@ -359,7 +359,9 @@ def attention_kv4(out: torch.Tensor, q: torch.Tensor, cache: KV4Cache, layer: in
     S, n, heads, hd = shape
     if not isinstance(layer, int) or not 0 <= layer < cache.layers:
         _layer(cache, layer)
-    qs, os_ = _rows(q, "q", shape, dtype, dev, True), _rows(out, "out", shape, dtype, dev)
+    qs, os_ = q.stride(), out.stride()
+    if out.shape != shape or out.dtype is not dtype or q.get_device() != dev or out.get_device() != dev or qs[3] != 1 or os_[3] != 1:
+        _rows(q, "q", shape, dtype, dev, True), _rows(out, "out", shape, dtype, dev)          # says what is wrong, or that nothing is (no element)
     flat = out.is_contiguous()
     if not flat:
         _spread(out, "out")
