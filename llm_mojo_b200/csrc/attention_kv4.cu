@@ -22,7 +22,9 @@ namespace {
 //      first column, which gives the even columns of o, and (0, p) in its second, the odd ones; with more rows two byte permutations
 //      of every four values make pairs of keys.
 // code x scale is exact in f16.  q is brought into f16's range by a power of two per row (exact for bf16; an fp32 row takes two columns, its
-// upper and its lower 11 bits), P is scaled by a power of two into the rest of f16's range and, for fp32, split alike.  P^T comes out of the accumulators of
+// upper and its lower 11 bits), P is scaled by a power of two into the rest of f16's range and, for fp32, split alike.  In bf16 a weight is so off by
+// up to 2^-11 of itself, an eighth of what the result's own rounding is (one below f16's normal numbers by 2^-32 of their sum); the sum that it is
+// divided by is taken of the fp32 weights.  P^T comes out of the accumulators of
 // S^T as the second product's other operand by a transposition within the warp (movmatrix).
 //
 // Each warp has a ring of its own of key tiles, filled by untiled bulk copies (a tile is contiguous in each of the four tensors), and

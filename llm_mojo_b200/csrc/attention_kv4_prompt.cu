@@ -7,8 +7,9 @@
 //   - no TMA: warps 12 and 15 read the codes and scales of a block's keys and values (from whichever slot keeps the page), turn them into f16
 //     and write the swizzled tiles that the tensor core reads (code x scale is exact in f16: cvt and a multiplication for two values);
 //   - the output warpgroup brings the next item's rows of q into f16's range by a power of two each (exact) and writes their tiles;
-//   - P is f16, up to 2^15: the maximum lags by up to 2^8, the rest of the range goes to small weights.
-// 16 x 12 heads, ragged prompts of up to 1000 tokens: 73 us; the kernel for few rows (mma.sync, 32 rows a warp) takes 237 us there.  All prompts
+//   - P is f16, up to 2^15: the maximum lags by up to 2^8, the rest of the range goes to small weights.  A weight is off by up to 2^-11 of itself, an
+//     eighth of what a bf16 result's own rounding is, or, below f16's normal numbers, by 2^-32 of their sum.
+// 16 x 12 heads, ragged prompts of up to 1000 tokens: 72 us; the kernel for few rows (mma.sync, 32 rows a warp) takes 158 us there.  All prompts
 // 1024 long: 90 us, the causal forward kernel on bf16 keys 69.  A softmax warp's chain (scores, maximum, 2^x, P) per block bounds both; the conversion
 // of the codes adds 6 us.
 #include "kv4.cuh"

@@ -63,7 +63,8 @@ template <int HD> struct AppendGroup { static constexpr int value = HD <= 32 ? 4
 // a half; r takes one Newton step from the approximate one, which is the correctly rounded one for all eight significands that scales have.
 // The negative quotient is made (with -r for r) and the codes' signs are turned back: the correction adds a zero to q = x r = -0 and would make
 // it +0; to -q it adds one of q's sign, so that zeros keep theirs.
-// Instructions bound this kernel (about 100 for 16 values).
+// The ALU pipe is the busiest unit (67 % of its cycles, issue slots 59 %; about 165 instructions for 16 values, idle lanes among them): 16 x 25 heads,
+// prompts of 500 to 1000 tokens, 100 MB: 28.7 us in bf16, 35.1 in fp32 (179 MB).
 template <typename T, int HD, bool VEC>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Desc d, int layer, const T* __restrict__ k, const T* __restrict__ v,
                                                          const int* __restrict__ start, const int* __restrict__ counts, int n, Divisor by_heads, RowStrides sk, RowStrides sv) {

@@ -56,7 +56,7 @@ def _status_at(device: torch.device, index: int) -> int:
 
 class KV4Cache:
     """The four tensors of a cache (see the module), checked once.  Layers and slots may be strided views of larger caches (every third
-    slot, some of the layers); heads, tokens and values lie densely, every row 16-byte aligned."""
+    slot, some of the layers); heads, tokens and values lie densely, every row 16-byte aligned.  No two of the four share memory."""
 
     __slots__ = ("k_codes", "k_scales", "v_codes", "v_scales", "k_unit", "v_unit", "layers", "slots", "kv_heads", "capacity", "head_size",
                  "device", "index", "_desc", "_status")
@@ -297,7 +297,7 @@ def kv4_values(k_out: torch.Tensor, v_out: torch.Tensor, cache: KV4Cache, layer:
                pages: Optional[torch.Tensor] = None) -> None:
     """Reads back what the cache holds: ``k_out``, ``v_out`` [slots, n, kv_heads, head_size] (bf16, in which every value is exact, or fp32) of
     the positions ``start[s] + i`` of one layer, or [layers, slots, ...] of all layers (``layer`` None).  Positions outside the cache read as
-    zeros, pages whose entry in ``pages`` names no slot as NaN."""
+    zeros, pages whose entry in ``pages`` names no slot as NaN.  The outputs share no memory."""
     dtype, dev, shape = k_out.dtype, cache.index, k_out.shape
     lead = (cache.slots,) if layer is not None else (cache.layers, cache.slots)
     if len(shape) != len(lead) + 3 or shape[:-3] != lead or shape[-2] != cache.kv_heads or shape[-1] != cache.head_size:
@@ -419,7 +419,7 @@ def kv4_reorder(cache: KV4Cache, pages: torch.Tensor, lens: torch.Tensor, parent
     """The cache follows a beam search: slot b K + j of item b becomes what slot b K + ``parents[b, j]`` was (``parents`` int32 [items, K],
     items x K = slots), in place and in every layer.  Entries of ``pages`` for whole pages and ``lens`` are permuted; of the keys and values
     only the page that is being filled is copied, at most 63 tokens.  Entries for pages that are not full name the slot itself.  A parent
-    outside 0 .. K - 1 counts as j itself; lengths beyond the capacity count as the capacity.
+    outside 0 .. K - 1 counts as j itself; lengths beyond the capacity count as the capacity.  The three tables share no memory.
 
     The parents that one item names have one length, as beams that grew together have: the page in which a shorter one ends may be a full
     page of a longer one, shared by that one's other children, and the shorter one's child goes on writing into it.

@@ -8,7 +8,8 @@
     python profile_kernels.py nvfp4       # NVFP4 operands (maxima, both orientations) and block-scaled GEMMs, 8192 x 1600 x 6400
     python profile_kernels.py fp8b        # block-scaled FP8 operands (both orientations) and GEMMs, 8192 x 1280 x 5120
     python profile_kernels.py lmhead      # LM-head GEMM on 8192 rows + fused softmax/cross-entropy
-    python profile_kernels.py kv4         # attention over the 4-bit cache: 256 x 16 heads of 1000 tokens, shared heads of 32000, a prompt; append, read back, reorder
+    python profile_kernels.py kv4         # attention over the 4-bit cache, ragged lengths: 256 x 16 heads of up to 1024 tokens, shared heads of 32001, prompts, fp32;
+                                          # append, read back, reorder
     python profile_kernels.py beam        # beam selection, 48 items of 8 beams over 50257 fp32 logits
     python profile_kernels.py layernorm   # LayerNorm forward + backward on 65536 x 768
     python profile_kernels.py fusedpull   # a layer GEMM that pulls its own weight (four emulated owners) with its copier warps
@@ -21,6 +22,7 @@ plain first and then under `ncu -k regex:<kernel> -c <n>` with the same command 
 that times the whole model is profile_gpt2.py (reference: profile_gpt2.mojo / profile_gpt2cu.py).
 """
 import argparse
+import random
 
 import torch
 
@@ -105,21 +107,30 @@ def case_kv4(reps):
             t.random_(40, 64)
         return c
 
-    def attend(c, heads, n, length):
-        q = torch.randn(c.slots, n, heads, c.head_size, device="cuda").bfloat16()
-        ops.attention_kv4(torch.empty_like(q), q, c, 0, torch.full((c.slots,), length, dtype=torch.int32, device="cuda"))
+    def ragged(S, longest):                                # the longest first, the others between half of it and all of it
+        r = random.Random(longest * 1000 + S)
+        return [longest] + [r.randint(longest // 2, longest) for _ in range(S - 1)]
 
-    wide, shared, prompt, beams = cache(1, 256, 16, 1000, 64), cache(1, 4, 8, 32000, 128), cache(1, 16, 12, 1000, 64), cache(24, 64, 16, 800, 64)
-    qkv = torch.randn(16, 1000, 3, 12, 64, device="cuda").bfloat16()
+    def ints(v):
+        return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+    def attend(c, heads, longest, new=1, dtype=torch.bfloat16):
+        q, lens = torch.randn(c.slots, new, heads, c.head_size, device="cuda").to(dtype), ragged(c.slots, longest)
+        ops.attention_kv4(torch.empty_like(q), q, c, 0, ints(lens), counts=ints(lens) if new > 1 else None)
+
+    wide, shared, prompt, beams = cache(1, 256, 16, 1024, 64), cache(1, 4, 8, 32001, 128), cache(1, 16, 12, 1000, 64), cache(24, 64, 16, 800, 64)
+    single, long_prompts = cache(1, 16, 16, 1500, 96), cache(1, 16, 25, 1000, 64)
+    qkv = torch.randn(16, 1000, 3, 25, 64, device="cuda").bfloat16()
     ko, vo = (torch.empty(24, 64, 64, 16, 64, device="cuda", dtype=torch.bfloat16) for _ in range(2))
     pages, lens = beams.own_pages(), torch.full((64,), 800, dtype=torch.int32, device="cuda")
     parents = torch.randint(0, 8, (8, 8), dtype=torch.int32, device="cuda")
-    zeros = torch.zeros(64, dtype=torch.int32, device="cuda")
+    zeros, counts = torch.zeros(64, dtype=torch.int32, device="cuda"), ints(ragged(16, 1000))
     for _ in range(reps):
-        attend(wide, 16, 1, 1000)
-        attend(shared, 32, 1, 32000)
+        attend(wide, 16, 1024)
+        attend(shared, 32, 32001)
         attend(prompt, 12, 1000, 1000)
-        ops.kv4_append(prompt, 0, qkv[:, :, 1], qkv[:, :, 2], zeros[:16])
+        attend(single, 16, 1500, dtype=torch.float32)
+        ops.kv4_append(long_prompts, 0, qkv[:, :, 1], qkv[:, :, 2], zeros[:16], counts=counts)
         ops.kv4_reorder(beams, pages, lens, parents)
         ops.kv4_values(ko, vo, beams, None, zeros)
 
