@@ -225,9 +225,9 @@ def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
         w, d = t.element_size(), list(d)
         while d and d[-1][1] == w:
             w *= d.pop()[0]
-        at = torch.tensor([p])
+        at = torch.tensor([p], device="cpu")
         for n, s in d:
-            at = (at.view(-1, 1) + torch.arange(n) * s).view(-1)
+            at = (at.view(-1, 1) + torch.arange(n, device="cpu") * s).view(-1)
         starts.append(at)
         width.append(w)
     at = starts[0].sort().values

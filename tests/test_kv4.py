@@ -362,3 +362,37 @@ def test_tables_of_a_reorder_share_no_memory():
     for pages, lens, parents in ((0, 11, 20), (5, 0, 20), (0, 20, 11), (9, 20, 4), (20, 0, 5), (20, 5, 0), (20, 0, 0)):
         with pytest.raises(ValueError, match="share memory"):
             ops.kv4_reorder(c, at(pages, 6, 2), at(lens, 6), at(parents, 2, 3))
+
+
+def test_memory_in_common_is_decided_exactly():
+    """Against sets of addresses: nested strides in any order, shifted copies of one layout and two layouts, types of other sizes; on the host
+    whatever the default device is."""
+    import random
+    r, memory, seen = random.Random(0), torch.zeros(4000, dtype=torch.uint8), set()
+
+    def layout():
+        shape = [r.randint(1, 4) for _ in range(r.randint(1, 4))]
+        strides, span = [0] * len(shape), 1
+        for i in r.sample(range(len(shape)), len(shape)):
+            strides[i] = span + r.choice([0, 0, 1, 4])
+            span += strides[i] * (shape[i] - 1)
+        return shape, strides, span
+
+    def addresses(t):
+        at = [t.data_ptr()]
+        for n, s in zip(t.shape, t.stride()):
+            at = [a + i * s * t.element_size() for a in at for i in range(n)]
+        return {a + b for a in at for b in range(t.element_size())}
+    with torch.device("meta"):
+        for _ in range(4000):
+            one, d1 = layout(), r.choice([torch.uint8, torch.bfloat16, torch.float32])
+            two, d2 = (one, d1) if r.random() < 0.5 else (layout(), r.choice([torch.uint8, torch.bfloat16]))
+            if max(one[2] * d1.itemsize, two[2] * d2.itemsize) > 1500:
+                continue
+            first = r.randint(0, 300)
+            a = memory.view(d1).as_strided(*one[:2], first)
+            b = memory.view(d2).as_strided(*two[:2], max(0, first * d1.itemsize // d2.itemsize + r.randint(-60, 60)))
+            want = bool(addresses(a) & addresses(b))
+            seen.add((one is two, want))
+            assert ops.kv4._meet(a, b) == want, (a.shape, a.stride(), b.shape, b.stride(), b.data_ptr() - a.data_ptr())
+    assert len(seen) == 4
